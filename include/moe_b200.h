@@ -372,6 +372,54 @@ MOE_API int moe_fused_expert_rows(const void* x, int x_dtype, int64_t rows, int6
                                   void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* --------------------------------------------------------------------------
+ * 4-bit expert weights with group scales (no reference counterpart).
+ *   W[n, k] = (q[n, k] - 8) * s[n, k / group_size],  q in 0..15
+ * A weight row of K values is K / 2 bytes: byte b holds q[2b] in its low and
+ * q[2b + 1] in its high nibble. s is bf16 or fp16; group_size is 32, 64 or
+ * 128 and divides K. Weights are K-major as above: w13 [E, 2I, H / 2] bytes
+ * with scales [E, 2I, H / group_size], w2 [E, H, I / 2] with [E, H,
+ * I / group_size]. Activations and scales share their type (bf16 or fp16); up
+ * to 1024 experts.
+ *
+ * moe_quant_int4_groups: rows [rows, cols] (bf16/fp16/fp32) -> q and s with
+ * s = absmax / 7 of each group (fp32 quotient, rounded to the scales' type)
+ * and q = 8 + clamp(rint(w / s), -8, 7), the quotient exact and rounded half
+ * to even; q = 8 where s is 0. A group that holds a NaN or an infinity, or
+ * whose scale is too large for its type, gets a NaN scale and q = 8.
+ * moe_dequant_int4_groups: the values that q and s stand for, each product
+ * rounded once to dst_dtype.
+ *
+ * moe_grouped_matmul_int4: x [num_rows, k] holds the rows of expert 0, then
+ * those of expert 1, ...; group_sizes [E] (int32/int64) counts them (negative
+ * counts are empty, counts past num_rows are cut off). out[r, c] =
+ * sum_k x[r, k] W[e(r), c, k], in x's type; rows behind the last group are zero.
+ *
+ * moe_fused_mlp_int4 / moe_fused_experts_int4: the layer in its pre-routed and
+ * top-k forms (moe_fused_mlp, moe_fused_experts) with 4-bit weights. h is
+ * rounded to x's type before the down projection. Tokens' rows are combined
+ * in slot order, so results do not differ from run to run.
+ * -------------------------------------------------------------------------- */
+MOE_API int moe_quant_int4_groups(const void* src, int src_dtype, int64_t rows, int64_t cols, int group_size,
+                                  uint8_t* dst, void* dst_scale, int scale_dtype, void* stream);
+MOE_API int moe_dequant_int4_groups(const uint8_t* src, const void* scale, int scale_dtype, int64_t rows,
+                                    int64_t cols, int group_size, void* dst, int dst_dtype, void* stream);
+MOE_API int moe_grouped_matmul_int4(const void* x, int dtype, int64_t num_rows, int64_t k, const uint8_t* w,
+                                    const void* w_scale, int group_size, int num_experts, int64_t n,
+                                    const void* group_sizes, int gs_dtype, void* out, void* stream);
+MOE_API size_t moe_fused_mlp_int4_workspace_size(int64_t num_tokens, int64_t inter, int num_experts);
+MOE_API int moe_fused_mlp_int4(const void* x, int dtype, int64_t num_tokens, int64_t hidden, const uint8_t* w13,
+                               const void* w13_scale, const uint8_t* w2, const void* w2_scale, int group_size,
+                               int num_experts, int64_t inter, const void* group_sizes, int gs_dtype, void* out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+MOE_API size_t moe_fused_experts_int4_workspace_size(int64_t num_tokens, int64_t hidden, int64_t inter,
+                                                     int num_experts, int top_k);
+MOE_API int moe_fused_experts_int4(const void* x, int dtype, int64_t num_tokens, int64_t hidden, const uint8_t* w13,
+                                   const void* w13_scale, const uint8_t* w2, const void* w2_scale, int group_size,
+                                   int num_experts, int64_t inter, const float* topk_weights,
+                                   const int32_t* topk_ids, int top_k, void* y, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------------------------------
  * Expert parallelism over NVLink peer memory (no reference counterpart: the
  * reference has no distributed code). Rank r of W owns experts
  * [r*EL, (r+1)*EL). Each rank allocates once (moe_ipc_malloc) a receive

@@ -69,6 +69,13 @@ SIGNATURES = {
                                 _sz, _p]),
     "moe_fused_expert_rows_workspace_size": (_sz, [_i64, _i64, _i64, _i, _i, _i]),
     "moe_fused_expert_rows": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i, _i64, _p, _p, _p, _p, _p, _sz, _p]),
+    "moe_quant_int4_groups": (_i, [_p, _i, _i64, _i64, _i, _p, _p, _i, _p]),
+    "moe_dequant_int4_groups": (_i, [_p, _p, _i, _i64, _i64, _i, _p, _i, _p]),
+    "moe_grouped_matmul_int4": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i, _i64, _p, _i, _p, _p]),
+    "moe_fused_mlp_int4_workspace_size": (_sz, [_i64, _i64, _i]),
+    "moe_fused_mlp_int4": (_i, [_p, _i, _i64, _i64, _p, _p, _p, _p, _i, _i, _i64, _p, _i, _p, _p, _sz, _p]),
+    "moe_fused_experts_int4_workspace_size": (_sz, [_i64, _i64, _i64, _i, _i]),
+    "moe_fused_experts_int4": (_i, [_p, _i, _i64, _i64, _p, _p, _p, _p, _i, _i, _i64, _p, _p, _i, _p, _p, _sz, _p]),
 }
 
 _lib = None

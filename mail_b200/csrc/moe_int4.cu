@@ -1,0 +1,675 @@
+// Experts with 4-bit weights (int4.cuh has the format): quantising and reading
+// back, products grouped by expert for few rows an expert, and the C entry
+// points of the 4-bit operators.
+#include <algorithm>
+
+#include "common.cuh"
+#include "int4.cuh"
+#include "rows.cuh"
+
+namespace moe {
+namespace {
+
+using u4::Act;
+
+// ---------------------------------------------------------------------------
+// Quantising with group scales.
+//   s = T(absmax / 7)  (fp32 quotient, then the scales' type)
+//   q = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0
+// GROUP / 8 lanes share a group; a lane loads eight weights and stores their
+// four bytes. The rounding is that of the exact quotient (half to even): the
+// sign of w - (f + 1/2) s, one fma and so exact, decides between f and f + 1
+// where f is the floor of the rounded quotient.
+// A group with a NaN or an infinity, or whose scale is too large for its type,
+// gets a NaN scale and q = 8, so what it stands for shows as NaN.
+__device__ __forceinline__ int nearest_step(float w, float s) {
+  const float f = floorf(__fdiv_rn(w, s));
+  const float side = fmaf(-(f + 0.5f), s, w);
+  const int i = (int)f;
+  const int up = side > 0.f || (side == 0.f && (i & 1)) ? 1 : 0;
+  return max(-8, min(7, i + up));
+}
+
+template <typename Tw, typename Ts, int GROUP>
+__global__ void __launch_bounds__(256) quant_groups_kernel(const Tw* __restrict__ src, int64_t n8,
+                                                           uint32_t* __restrict__ dst, Ts* __restrict__ scale) {
+  pdl_begin();
+  constexpr int kLanes = GROUP / 8;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;  // a multiple of kLanes: a group's lanes stay together
+  const int64_t last = (n8 + 31) / 32 * 32;                // whole warps take part in the shuffles
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < last; i += stride) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i < n8) rows::load8(src + i * 8, v);
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      amax = fmaxf(amax, fabsf(v[j]));
+      bad |= !isfinite(v[j]);
+    }
+    if (bad) amax = INFINITY;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    Ts st = Act<Ts>::from_float(__fdiv_rn(amax, 7.0f));
+    float s = Act<Ts>::to_float(st);
+    if (!isfinite(s)) {
+      st = Act<Ts>::from_float(NAN);
+      s = 0.f;
+    }
+    uint32_t word = 0x88888888u;
+    if (s > 0.f) {
+      word = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) word |= (uint32_t)(nearest_step(v[j], s) + 8) << (4 * j);
+    }
+    if (i < n8) {
+      dst[i] = word;
+      if (i % kLanes == 0) scale[i / kLanes] = st;
+    }
+  }
+}
+
+template <typename Ts, typename To, int GROUP>
+__global__ void __launch_bounds__(256) dequant_groups_kernel(const uint32_t* __restrict__ src,
+                                                             const Ts* __restrict__ scale, int64_t n8,
+                                                             To* __restrict__ dst) {
+  pdl_begin();
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t)gridDim.x * blockDim.x) {
+    const uint32_t w = src[i];
+    const float s = Act<Ts>::to_float(scale[i / (GROUP / 8)]);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * s;
+    rows::store8(dst + i * 8, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products grouped by expert, few rows an expert:
+//   out[r, n] = sum_k x[r, k] W[e(r), n, k]
+// SWIGLU: W holds I gate rows and I up rows and out[r, n] = silu(g) u.
+//
+// One CTA takes a strip of weight rows of one expert and all of the expert's
+// rows, eight at a time per mma (m16n8k16: sixteen weight rows by eight
+// tokens). Its eight warps are WM strips of sixteen weight rows by WK shares
+// of K; the shares are added through shared memory in the order of the warps,
+// so results do not depend on timing. With SWIGLU a strip's sixteen rows are
+// eight gate rows and the eight up rows that go with them.
+//
+// A lane (row g = lane / 4, t = lane % 4) loads GROUP / 4 consecutive k of its
+// two weight rows at a time, so that the four lanes of a row cover exactly one
+// group of scales: the products of a group are summed from the integers
+// q - 8, which 16-bit types hold exactly, and the fp32 sum is scaled once,
+// which rounds no weight.
+constexpr int kMvThreads = 256;
+constexpr int kMvWarps = kMvThreads / 32;
+constexpr int kMaxSlots = 1024;  // routed slots of the form that reads top-k ids
+
+struct MvParams {
+  const void* x;         // [.., K]
+  const uint8_t* w;      // [E, w_rows, K / 2]
+  const void* scale;     // [E, w_rows, K / group]
+  void* out;             // [rows, n_out]
+  int64_t K;
+  int n_out, w_rows;     // output features; weight rows of an expert (2 n_out with SWIGLU)
+  int E;
+  int wk;                // shares of K (1, 2, 4 or 8)
+  int out_f32;           // out is fp32, else the activations' type
+  // rows: either the top-k ids of `slots` slots (row r of x is slot / x_div, row
+  // of out is the slot), or counts of consecutive rows
+  const int32_t* ids;
+  int slots;
+  const void* counts;
+  int counts_is64;
+  int64_t total_rows;    // rows of out; those that no expert has are zeroed
+  const int32_t* row_map;  // counts form: row r reads x row row_map[r] / x_div (NULL: r)
+  int x_div;
+};
+
+template <typename T, int GROUP, int NT, bool SWIGLU>
+__global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p) {
+  pdl_begin();
+  constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
+  constexpr int kPer = 128 / GROUP;       // groups of a block of 128 k
+  constexpr int kTokens = 8 * NT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+  __shared__ int s_list[kMaxSlots];
+  __shared__ int s_part[kMaxSlots / 32];
+  __shared__ int64_t s_sum[kMvWarps];
+  __shared__ int64_t s_x[kTokens], s_o[kTokens];
+  __shared__ float s_red[kMvWarps][16][kTokens + 1];
+
+  const int wm = kMvWarps / p.wk;
+  const int strips = (p.n_out + (SWIGLU ? 7 : 15)) / (SWIGLU ? 8 : 16);
+  int e;
+  int64_t off = 0, cnt = 0;
+  if (p.ids) {
+    // this CTA stands for the slot blockIdx.y; the first slot of an expert
+    // works for all of them
+    const int me = blockIdx.y;
+    e = p.ids[me];
+    if (e < 0 || e >= p.E) return;
+    const int passes = (p.slots + kMvThreads - 1) / kMvThreads;
+    bool mine[kMaxSlots / kMvThreads];
+    int before[kMaxSlots / kMvThreads];
+    bool earlier = false;
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / kMvThreads; ++i) {
+      mine[i] = false;
+      before[i] = 0;
+      if (i < passes) {
+        const int s = i * kMvThreads + threadIdx.x;
+        mine[i] = s < p.slots && p.ids[s] == e;
+        earlier |= mine[i] && s < me;
+        const unsigned b = __ballot_sync(0xffffffffu, mine[i]);
+        before[i] = __popc(b & ((1u << lane) - 1));
+        if (lane == 0) s_part[i * kMvWarps + warp] = __popc(b);
+      }
+    }
+    if (__syncthreads_or(earlier)) return;
+    int run = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxSlots / kMvThreads; ++i) {
+      if (i < passes) {
+        for (int w = 0; w < kMvWarps; ++w) {
+          if (w == warp && mine[i]) s_list[run + before[i]] = i * kMvThreads + threadIdx.x;
+          run += s_part[i * kMvWarps + w];
+        }
+      }
+    }
+    cnt = run;
+    __syncthreads();
+  } else {
+    e = blockIdx.y;  // e == E: the rows that no expert has
+    int64_t sum = 0;
+    for (int i = threadIdx.x; i < min(e, p.E); i += kMvThreads) {
+      const int64_t c = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[i]
+                                      : (int64_t) static_cast<const int32_t*>(p.counts)[i];
+      sum += max(c, (int64_t)0);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    for (int w = 0; w < kMvWarps; ++w) off += s_sum[w];
+    off = min(off, p.total_rows);
+    if (e == p.E) {
+      const int es = p.out_f32 ? 4 : 2;
+      const int64_t n0 = (int64_t)blockIdx.x * wm * (SWIGLU ? 8 : 16);
+      const int64_t n1 = min((int64_t)p.n_out, n0 + wm * (SWIGLU ? 8 : 16));
+      for (int64_t r = off; r < p.total_rows; ++r)
+        for (int64_t n = n0 + threadIdx.x; n < n1; n += kMvThreads) {
+          if (es == 4) static_cast<float*>(p.out)[r * p.n_out + n] = 0.f;
+          else static_cast<uint16_t*>(p.out)[r * p.n_out + n] = 0;
+        }
+      return;
+    }
+    cnt = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[e]
+                        : (int64_t) static_cast<const int32_t*>(p.counts)[e];
+    cnt = max((int64_t)0, min(cnt, p.total_rows - off));
+    if (cnt == 0) return;
+  }
+
+  const int sm = warp / p.wk, share = warp % p.wk;  // strip of this warp, its share of K
+  const int strip = blockIdx.x * wm + sm;
+  const int blocks = (int)((p.K + 127) / 128);
+  const int b0 = (int)((int64_t)blocks * share / p.wk), b1 = (int)((int64_t)blocks * (share + 1) / p.wk);
+  // rows of W of this lane: row g and row g + 8 of the strip (rows past the
+  // end read the last row and are not stored)
+  int r0, r1;
+  if (SWIGLU) {
+    const int f = min(strip * 8 + g, p.n_out - 1);
+    r0 = f;
+    r1 = p.n_out + f;
+  } else {
+    r0 = min(strip * 16 + g, p.n_out - 1);
+    r1 = min(strip * 16 + g + 8, p.n_out - 1);
+  }
+  const int64_t groups = p.K / GROUP;
+  const int64_t row0 = (int64_t)e * p.w_rows + r0, row1 = (int64_t)e * p.w_rows + r1;
+  const uint8_t* w0 = p.w + row0 * (p.K / 2) + t * 4 * kWords;
+  const uint8_t* w1 = p.w + row1 * (p.K / 2) + t * 4 * kWords;
+  const T* sc0 = static_cast<const T*>(p.scale) + row0 * groups;
+  const T* sc1 = static_cast<const T*>(p.scale) + row1 * groups;
+  const T* x = static_cast<const T*>(p.x);
+
+  for (int64_t c0 = 0; c0 < cnt; c0 += kTokens) {
+    if (threadIdx.x < kTokens) {
+      const int64_t i = c0 + threadIdx.x;
+      int64_t xr = -1, orow = -1;
+      if (i < cnt) {
+        orow = p.ids ? (int64_t)s_list[i] : off + i;
+        xr = p.ids ? orow / p.x_div : (p.row_map ? (int64_t)(p.row_map[orow] / p.x_div) : orow);
+      }
+      s_x[threadIdx.x] = xr;
+      s_o[threadIdx.x] = orow;
+    }
+    __syncthreads();
+    float acc[NT][4];
+    const T* xp[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+      const int64_t xr = s_x[n * 8 + g];
+      xp[n] = xr >= 0 ? x + xr * p.K + t * 8 * kWords : nullptr;
+    }
+    if (strip < strips) {
+#pragma unroll 2
+      for (int b = b0; b < b1; ++b) {
+        uint32_t q0[kPer][kWords], q1[kPer][kWords];
+        float s0[kPer], s1[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int64_t grp = (int64_t)b * kPer + j;
+          const bool in = grp < groups;
+          s0[j] = in ? Act<T>::to_float(sc0[grp]) : 0.f;
+          s1[j] = in ? Act<T>::to_float(sc1[grp]) : 0.f;
+          const int64_t at = grp * (GROUP / 2);
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) q0[j][i] = q1[j][i] = 0x88888888u;
+          if (in) {
+            if constexpr (kWords == 4) {
+              *reinterpret_cast<uint4*>(q0[j]) = __ldg(reinterpret_cast<const uint4*>(w0 + at));
+              *reinterpret_cast<uint4*>(q1[j]) = __ldg(reinterpret_cast<const uint4*>(w1 + at));
+            } else if constexpr (kWords == 2) {
+              *reinterpret_cast<uint2*>(q0[j]) = __ldg(reinterpret_cast<const uint2*>(w0 + at));
+              *reinterpret_cast<uint2*>(q1[j]) = __ldg(reinterpret_cast<const uint2*>(w1 + at));
+            } else {
+              q0[j][0] = __ldg(reinterpret_cast<const uint32_t*>(w0 + at));
+              q1[j][0] = __ldg(reinterpret_cast<const uint32_t*>(w1 + at));
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int64_t grp = (int64_t)b * kPer + j;
+          const bool in = grp < groups;
+          float part[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            uint32_t a0[4], a1[4];
+            Act<T>::decode(q0[j][i], a0);
+            Act<T>::decode(q1[j][i], a1);
+            const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              uint32_t bx[4] = {0u, 0u, 0u, 0u};
+              if (in && xp[n]) u4::pair_up(*reinterpret_cast<const uint4*>(xp[n] + grp * GROUP + i * 8), bx);
+              Act<T>::mma(part[n], lo, bx[0], bx[1]);
+              Act<T>::mma(part[n], hi, bx[2], bx[3]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[n][0] = fmaf(s0[j], part[n][0], acc[n][0]);
+            acc[n][1] = fmaf(s0[j], part[n][1], acc[n][1]);
+            acc[n][2] = fmaf(s1[j], part[n][2], acc[n][2]);
+            acc[n][3] = fmaf(s1[j], part[n][3], acc[n][3]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s_red[warp][g][n * 8 + 2 * t] = acc[n][0];
+      s_red[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
+      s_red[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
+      s_red[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
+    }
+    __syncthreads();
+    // strip m, feature f, token n: the shares added in order
+    constexpr int kFeat = SWIGLU ? 8 : 16;
+    for (int i = threadIdx.x; i < wm * kFeat * kTokens; i += kMvThreads) {
+      const int f = i % kFeat, m = i / kFeat % wm, n = i / (kFeat * wm);
+      const int feat = (blockIdx.x * wm + m) * kFeat + f;
+      const int64_t orow = s_o[n];
+      if (orow < 0 || feat >= p.n_out) continue;
+      float v = 0.f, u = 0.f;
+      for (int k = 0; k < p.wk; ++k) {
+        v += s_red[m * p.wk + k][f][n];
+        if (SWIGLU) u += s_red[m * p.wk + k][f + 8][n];
+      }
+      if (SWIGLU) v = u4::silu_mul(v, u);
+      const int64_t at = orow * p.n_out + feat;
+      if (p.out_f32) static_cast<float*>(p.out)[at] = v;
+      else static_cast<T*>(p.out)[at] = Act<T>::from_float(v);
+    }
+    __syncthreads();
+  }
+}
+
+// y[t] = sum_j weight[t, j] * o[row of slot (t, j)], slots in order; a slot
+// whose id names no expert adds nothing. slot_row NULL: the row is the slot.
+template <typename T>
+__global__ void __launch_bounds__(256) int4_combine_kernel(const float* __restrict__ o,
+                                                           const int32_t* __restrict__ ids,
+                                                           const int32_t* __restrict__ slot_row,
+                                                           const float* __restrict__ weight, int64_t T8, int64_t H8,
+                                                           int k, int E, T* __restrict__ y) {
+  pdl_begin();
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < T8; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / H8, c = i % H8 * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < k; ++j) {
+      const int64_t s = t * k + j;
+      const int id = ids[s];
+      if (id < 0 || id >= E) continue;
+      const int64_t row = slot_row ? (int64_t)slot_row[s] : s;
+      const float w = weight[s];
+      float v[8];
+      rows::load8(o + row * H8 * 8 + c, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] = fmaf(w, v[q], acc[q]);
+    }
+    rows::store8(y + t * H8 * 8 + c, acc);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+bool act_ok(int dtype) { return dtype == MOE_BF16 || dtype == MOE_F16; }
+
+unsigned flat_grid(int64_t threads) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(threads, 256), (int64_t)num_sms() * 16));
+}
+
+template <typename Tw, typename Ts>
+int launch_quant(const void* src, int64_t n8, int group, void* dst, void* scale, cudaStream_t st) {
+#define MOE_QUANT(G)                                                                                      \
+  MOE_CUDA_TRY(launch_kernel(quant_groups_kernel<Tw, Ts, G>, dim3(flat_grid(n8)), dim3(256), 0, st,        \
+                             static_cast<const Tw*>(src), n8, static_cast<uint32_t*>(dst), static_cast<Ts*>(scale)))
+  if (group == 128) MOE_QUANT(128);
+  else if (group == 64) MOE_QUANT(64);
+  else MOE_QUANT(32);
+#undef MOE_QUANT
+  MOE_LAUNCH_CHECK("quant_groups_kernel");
+  return MOE_OK;
+}
+
+template <typename Ts, typename To>
+int launch_dequant(const void* src, const void* scale, int64_t n8, int group, void* dst, cudaStream_t st) {
+#define MOE_DEQUANT(G)                                                                                     \
+  MOE_CUDA_TRY(launch_kernel(dequant_groups_kernel<Ts, To, G>, dim3(flat_grid(n8)), dim3(256), 0, st,      \
+                             static_cast<const uint32_t*>(src), static_cast<const Ts*>(scale), n8, static_cast<To*>(dst)))
+  if (group == 128) MOE_DEQUANT(128);
+  else if (group == 64) MOE_DEQUANT(64);
+  else MOE_DEQUANT(32);
+#undef MOE_DEQUANT
+  MOE_LAUNCH_CHECK("dequant_groups_kernel");
+  return MOE_OK;
+}
+
+template <typename T, int GROUP, int NT, bool SWIGLU>
+int launch_rows_nt(MvParams p, cudaStream_t st) {
+  const int strips = (int)ceil_div(p.n_out, SWIGLU ? 8 : 16);
+  const int wm = kMvWarps / p.wk;
+  const dim3 grid((unsigned)ceil_div(strips, wm), (unsigned)(p.ids ? p.slots : p.E + 1));
+  MOE_CUDA_TRY(launch_kernel(int4_rows_kernel<T, GROUP, NT, SWIGLU>, grid, dim3(kMvThreads), 0, st, p));
+  MOE_LAUNCH_CHECK("int4_rows_kernel");
+  return MOE_OK;
+}
+
+template <typename T, int GROUP, bool SWIGLU>
+int launch_rows_group(MvParams p, int64_t rows, cudaStream_t st) {
+  // shares of K: as many as leave each warp two blocks of 128 k, fewer where
+  // the strips alone fill the device
+  const int64_t blocks = ceil_div(p.K, 128);
+  const int64_t units = ceil_div(p.n_out, SWIGLU ? 8 : 16) * std::min<int64_t>(p.E, rows);
+  p.wk = kMvWarps;
+  while (p.wk > 1 && (blocks < 2 * p.wk || units * p.wk > (int64_t)num_sms() * 64 * 4)) p.wk /= 2;
+  if (rows <= 8 || rows <= 2 * (int64_t)p.E) return launch_rows_nt<T, GROUP, 1, SWIGLU>(p, st);
+  return launch_rows_nt<T, GROUP, 4, SWIGLU>(p, st);
+}
+
+// rows: how many rows there are in all
+template <bool SWIGLU>
+int launch_rows(const MvParams& p, int dtype, int group, int64_t rows, cudaStream_t st) {
+  if (dtype == MOE_BF16) {
+    if (group == 128) return launch_rows_group<__nv_bfloat16, 128, SWIGLU>(p, rows, st);
+    if (group == 64) return launch_rows_group<__nv_bfloat16, 64, SWIGLU>(p, rows, st);
+    return launch_rows_group<__nv_bfloat16, 32, SWIGLU>(p, rows, st);
+  }
+  if (group == 128) return launch_rows_group<__half, 128, SWIGLU>(p, rows, st);
+  if (group == 64) return launch_rows_group<__half, 64, SWIGLU>(p, rows, st);
+  return launch_rows_group<__half, 32, SWIGLU>(p, rows, st);
+}
+
+struct LayerWs {
+  size_t h, o, align, sorted, slot_pos, gs, poff, table, align_bytes, bytes;
+  bool direct;  // the top-k ids are read by the product kernels themselves
+};
+LayerWs layer_ws(int64_t T, int64_t H, int64_t I, int E, int k) {
+  LayerWs w{};
+  const int64_t S = T * k;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = align_up(off + bytes, 256);
+    return o;
+  };
+  w.direct = S <= kMaxSlots;
+  w.h = take((size_t)S * I * 2);
+  w.o = take((size_t)S * H * sizeof(float));
+  if (!w.direct) {
+    w.align_bytes = moe_align_workspace_size(T, k, E, 1);
+    w.align = take(w.align_bytes);
+    w.sorted = take((size_t)moe_align_capacity(S, E, 1) * sizeof(int32_t));
+    w.slot_pos = take((size_t)S * sizeof(int32_t));
+    w.gs = take((size_t)E * sizeof(int32_t));
+    w.poff = take((size_t)(E + 1) * sizeof(int32_t));
+    w.table = take((size_t)moe_tile_table_ints(E, moe_align_capacity(S, E, 1)) * sizeof(int32_t));
+  }
+  w.bytes = off;
+  return w;
+}
+
+int check_weights(const char* fn, int dtype, int64_t k, int64_t n, int E, int group) {
+  MOE_CHECK_ARG(act_ok(dtype), "%s: 4-bit weights take bf16 or fp16 activations", fn);
+  MOE_CHECK_ARG(u4::group_ok(group), "%s: group size %d is not 32, 64 or 128", fn, group);
+  MOE_CHECK_ARG(k > 0 && k % group == 0 && k < (int64_t(1) << 30),
+                "%s: reduction length %lld must be a positive multiple of the group size %d", fn, (long long)k, group);
+  MOE_CHECK_ARG(n > 0 && n < (int64_t(1) << 30), "%s: bad output size %lld", fn, (long long)n);
+  MOE_CHECK_ARG(E > 0 && E <= 1024, "%s: num_experts %d outside [1, 1024]", fn, E);
+  return MOE_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_quant_int4_groups(const void* src, int src_dtype, int64_t rows, int64_t cols, int group_size,
+                                     uint8_t* dst, void* dst_scale, int scale_dtype, void* stream) {
+  MOE_CHECK_ARG(src_dtype == MOE_BF16 || src_dtype == MOE_F16 || src_dtype == MOE_F32,
+                "moe_quant_int4_groups: source must be bf16, fp16 or fp32");
+  MOE_CHECK_ARG(act_ok(scale_dtype), "moe_quant_int4_groups: scales must be bf16 or fp16");
+  MOE_CHECK_ARG(u4::group_ok(group_size), "moe_quant_int4_groups: group size %d is not 32, 64 or 128", group_size);
+  MOE_CHECK_ARG(rows >= 0 && cols > 0 && cols % group_size == 0,
+                "moe_quant_int4_groups: columns (%lld) must be a positive multiple of the group size %d",
+                (long long)cols, group_size);
+  if (rows == 0) return MOE_OK;
+  MOE_CHECK_ARG(src && dst && dst_scale, "moe_quant_int4_groups: NULL pointer");
+  MOE_CHECK_ARG((uintptr_t)src % 16 == 0 && (uintptr_t)dst % 4 == 0,
+                "moe_quant_int4_groups: source must be 16-byte and output 4-byte aligned");
+  const int64_t n8 = rows * cols / 8;
+  cudaStream_t st = as_stream(stream);
+  if (scale_dtype == MOE_BF16) {
+    if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
+    if (src_dtype == MOE_F16) return launch_quant<__half, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
+    return launch_quant<float, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
+  }
+  if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __half>(src, n8, group_size, dst, dst_scale, st);
+  if (src_dtype == MOE_F16) return launch_quant<__half, __half>(src, n8, group_size, dst, dst_scale, st);
+  return launch_quant<float, __half>(src, n8, group_size, dst, dst_scale, st);
+}
+
+extern "C" int moe_dequant_int4_groups(const uint8_t* src, const void* scale, int scale_dtype, int64_t rows,
+                                       int64_t cols, int group_size, void* dst, int dst_dtype, void* stream) {
+  MOE_CHECK_ARG(dst_dtype == MOE_BF16 || dst_dtype == MOE_F16 || dst_dtype == MOE_F32,
+                "moe_dequant_int4_groups: output must be bf16, fp16 or fp32");
+  MOE_CHECK_ARG(act_ok(scale_dtype), "moe_dequant_int4_groups: scales must be bf16 or fp16");
+  MOE_CHECK_ARG(u4::group_ok(group_size), "moe_dequant_int4_groups: group size %d is not 32, 64 or 128", group_size);
+  MOE_CHECK_ARG(rows >= 0 && cols > 0 && cols % group_size == 0,
+                "moe_dequant_int4_groups: columns (%lld) must be a positive multiple of the group size %d",
+                (long long)cols, group_size);
+  if (rows == 0) return MOE_OK;
+  MOE_CHECK_ARG(src && scale && dst, "moe_dequant_int4_groups: NULL pointer");
+  MOE_CHECK_ARG((uintptr_t)src % 4 == 0 && (uintptr_t)dst % 16 == 0,
+                "moe_dequant_int4_groups: source must be 4-byte and output 16-byte aligned");
+  const int64_t n8 = rows * cols / 8;
+  cudaStream_t st = as_stream(stream);
+  if (scale_dtype == MOE_BF16) {
+    if (dst_dtype == MOE_BF16) return launch_dequant<__nv_bfloat16, __nv_bfloat16>(src, scale, n8, group_size, dst, st);
+    if (dst_dtype == MOE_F16) return launch_dequant<__nv_bfloat16, __half>(src, scale, n8, group_size, dst, st);
+    return launch_dequant<__nv_bfloat16, float>(src, scale, n8, group_size, dst, st);
+  }
+  if (dst_dtype == MOE_BF16) return launch_dequant<__half, __nv_bfloat16>(src, scale, n8, group_size, dst, st);
+  if (dst_dtype == MOE_F16) return launch_dequant<__half, __half>(src, scale, n8, group_size, dst, st);
+  return launch_dequant<__half, float>(src, scale, n8, group_size, dst, st);
+}
+
+extern "C" int moe_grouped_matmul_int4(const void* x, int dtype, int64_t num_rows, int64_t k, const uint8_t* w,
+                                       const void* w_scale, int group_size, int num_experts, int64_t n,
+                                       const void* group_sizes, int gs_dtype, void* out, void* stream) {
+  MOE_TRY(check_weights("moe_grouped_matmul_int4", dtype, k, n, num_experts, group_size));
+  MOE_CHECK_ARG(gs_dtype == MOE_I32 || gs_dtype == MOE_I64, "moe_grouped_matmul_int4: group sizes must be int32 or int64");
+  MOE_CHECK_ARG(num_rows >= 0 && num_rows < (int64_t(1) << 31), "moe_grouped_matmul_int4: bad row count");
+  if (num_rows == 0) return MOE_OK;
+  MOE_CHECK_ARG(x && w && w_scale && group_sizes && out, "moe_grouped_matmul_int4: NULL pointer");
+  MOE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)out % 16 == 0,
+                "moe_grouped_matmul_int4: pointers must be 16-byte aligned");
+  MvParams p{};
+  p.x = x;
+  p.w = w;
+  p.scale = w_scale;
+  p.out = out;
+  p.K = k;
+  p.n_out = (int)n;
+  p.w_rows = (int)n;
+  p.E = num_experts;
+  p.counts = group_sizes;
+  p.counts_is64 = gs_dtype == MOE_I64;
+  p.total_rows = num_rows;
+  p.x_div = 1;
+  return launch_rows<false>(p, dtype, group_size, num_rows, as_stream(stream));
+}
+
+extern "C" size_t moe_fused_experts_int4_workspace_size(int64_t num_tokens, int64_t hidden, int64_t inter,
+                                                        int num_experts, int top_k) {
+  if (num_tokens < 0 || hidden <= 0 || inter <= 0 || num_experts <= 0 || top_k <= 0) return 0;
+  return layer_ws(num_tokens, hidden, inter, num_experts, top_k).bytes;
+}
+
+extern "C" int moe_fused_experts_int4(const void* x, int dtype, int64_t num_tokens, int64_t hidden,
+                                      const uint8_t* w13, const void* w13_scale, const uint8_t* w2,
+                                      const void* w2_scale, int group_size, int num_experts, int64_t inter,
+                                      const float* topk_weights, const int32_t* topk_ids, int top_k, void* y,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  MOE_TRY(check_weights("moe_fused_experts_int4", dtype, hidden, inter, num_experts, group_size));
+  MOE_TRY(check_weights("moe_fused_experts_int4", dtype, inter, hidden, num_experts, group_size));
+  MOE_CHECK_ARG(num_tokens >= 0 && top_k > 0 && num_tokens * top_k < (int64_t(1) << 31),
+                "moe_fused_experts_int4: bad sizes");
+  if (num_tokens == 0) return MOE_OK;
+  MOE_CHECK_ARG(x && w13 && w13_scale && w2 && w2_scale && topk_weights && topk_ids && y,
+                "moe_fused_experts_int4: NULL pointer");
+  MOE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w13 % 16 == 0 && (uintptr_t)w2 % 16 == 0 && (uintptr_t)y % 16 == 0,
+                "moe_fused_experts_int4: pointers must be 16-byte aligned");
+  const LayerWs w = layer_ws(num_tokens, hidden, inter, num_experts, top_k);
+  if (workspace_bytes < w.bytes || !workspace)
+    return set_error(MOE_ERR_WORKSPACE, "moe_fused_experts_int4: workspace %zu < %zu bytes", workspace_bytes, w.bytes);
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t st = as_stream(stream);
+  const int64_t S = num_tokens * top_k;
+  MvParams p{};
+  p.E = num_experts;
+  p.total_rows = S;
+  p.x_div = top_k;
+  if (w.direct) {
+    p.ids = topk_ids;
+    p.slots = (int)S;
+  } else {
+    int32_t* sorted = reinterpret_cast<int32_t*>(ws + w.sorted);
+    MOE_TRY(moe_align(topk_ids, num_tokens, top_k, num_experts, 1, sorted, reinterpret_cast<int32_t*>(ws + w.slot_pos),
+                      reinterpret_cast<int32_t*>(ws + w.gs), reinterpret_cast<int32_t*>(ws + w.poff),
+                      reinterpret_cast<int32_t*>(ws + w.table), ws + w.align, w.align_bytes, stream));
+    p.counts = ws + w.gs;
+    p.row_map = sorted;
+  }
+  p.x = x;
+  p.w = w13;
+  p.scale = w13_scale;
+  p.out = ws + w.h;
+  p.K = hidden;
+  p.n_out = (int)inter;
+  p.w_rows = (int)(2 * inter);
+  MOE_TRY(launch_rows<true>(p, dtype, group_size, S, st));
+  p.x = ws + w.h;
+  p.w = w2;
+  p.scale = w2_scale;
+  p.out = ws + w.o;
+  p.out_f32 = 1;
+  p.K = inter;
+  p.n_out = p.w_rows = (int)hidden;
+  p.row_map = nullptr;
+  p.x_div = 1;
+  MOE_TRY(launch_rows<false>(p, dtype, group_size, S, st));
+  const int64_t h8 = hidden / 8;
+  const int32_t* slot_row = w.direct ? nullptr : reinterpret_cast<const int32_t*>(ws + w.slot_pos);
+  const float* o = reinterpret_cast<const float*>(ws + w.o);
+  if (dtype == MOE_BF16)
+    MOE_CUDA_TRY(launch_kernel(int4_combine_kernel<__nv_bfloat16>, dim3(flat_grid(num_tokens * h8)), dim3(256), 0, st,
+                               o, topk_ids, slot_row, topk_weights, num_tokens * h8, h8, top_k, num_experts,
+                               static_cast<__nv_bfloat16*>(y)));
+  else
+    MOE_CUDA_TRY(launch_kernel(int4_combine_kernel<__half>, dim3(flat_grid(num_tokens * h8)), dim3(256), 0, st, o,
+                               topk_ids, slot_row, topk_weights, num_tokens * h8, h8, top_k, num_experts,
+                               static_cast<__half*>(y)));
+  MOE_LAUNCH_CHECK("int4_combine_kernel");
+  return MOE_OK;
+}
+
+extern "C" size_t moe_fused_mlp_int4_workspace_size(int64_t num_tokens, int64_t inter, int num_experts) {
+  if (num_tokens < 0 || inter <= 0 || num_experts <= 0) return 0;
+  return align_up((size_t)num_tokens * inter * 2, 256);
+}
+
+extern "C" int moe_fused_mlp_int4(const void* x, int dtype, int64_t num_tokens, int64_t hidden, const uint8_t* w13,
+                                  const void* w13_scale, const uint8_t* w2, const void* w2_scale, int group_size,
+                                  int num_experts, int64_t inter, const void* group_sizes, int gs_dtype, void* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  MOE_TRY(check_weights("moe_fused_mlp_int4", dtype, hidden, inter, num_experts, group_size));
+  MOE_TRY(check_weights("moe_fused_mlp_int4", dtype, inter, hidden, num_experts, group_size));
+  MOE_CHECK_ARG(gs_dtype == MOE_I32 || gs_dtype == MOE_I64, "moe_fused_mlp_int4: group sizes must be int32 or int64");
+  MOE_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t(1) << 31), "moe_fused_mlp_int4: bad row count");
+  if (num_tokens == 0) return MOE_OK;
+  MOE_CHECK_ARG(x && w13 && w13_scale && w2 && w2_scale && group_sizes && out, "moe_fused_mlp_int4: NULL pointer");
+  MOE_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)w13 % 16 == 0 && (uintptr_t)w2 % 16 == 0 && (uintptr_t)out % 16 == 0,
+                "moe_fused_mlp_int4: pointers must be 16-byte aligned");
+  const size_t need = moe_fused_mlp_int4_workspace_size(num_tokens, inter, num_experts);
+  if (workspace_bytes < need || !workspace)
+    return set_error(MOE_ERR_WORKSPACE, "moe_fused_mlp_int4: workspace %zu < %zu bytes", workspace_bytes, need);
+  cudaStream_t st = as_stream(stream);
+  MvParams p{};
+  p.E = num_experts;
+  p.total_rows = num_tokens;
+  p.x_div = 1;
+  p.counts = group_sizes;
+  p.counts_is64 = gs_dtype == MOE_I64;
+  p.x = x;
+  p.w = w13;
+  p.scale = w13_scale;
+  p.out = workspace;
+  p.K = hidden;
+  p.n_out = (int)inter;
+  p.w_rows = (int)(2 * inter);
+  MOE_TRY(launch_rows<true>(p, dtype, group_size, num_tokens, st));
+  p.x = workspace;
+  p.w = w2;
+  p.scale = w2_scale;
+  p.out = out;
+  p.K = inter;
+  p.n_out = p.w_rows = (int)hidden;
+  return launch_rows<false>(p, dtype, group_size, num_tokens, st);
+}

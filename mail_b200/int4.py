@@ -1,0 +1,246 @@
+"""Experts with 4-bit weights and group scales (w4a16).
+
+A weight row of K values is stored as K / 2 bytes and K / group_size scales:
+
+    W[n, k] = (q[n, k] - 8) * scale[n, k // group_size],   q in 0..15
+
+byte b of the row holds q[2b] in its low and q[2b + 1] in its high nibble;
+group_size is 32, 64 or 128 and divides K; the scales are in the activations'
+type (bf16 or fp16). Expert weights keep the framework's "(E, K, N)" logical
+layout with K-major storage, so a 4-bit w13 is a uint8 [E, H / 2, 2I] view of
+contiguous [E, 2I, H / 2] bytes with scales [E, 2I, H / group_size], and w2 is
+[E, I / 2, H] with scales [E, H, I / group_size]. `fused_moe_mlp` and
+`fused_moe_mlp_from_logits` take such weights with scales=(w13_scale, w2_scale).
+
+Every op runs the kernels of libmoe_b200.so on the current stream of its
+tensors' device; there is no CPU or PyTorch fallback.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib
+from .moe import _check_shapes, _code, _require_cuda, _stream, _workspace, kmajor
+
+GROUP_SIZES = (32, 64, 128)
+_ACT = (torch.bfloat16, torch.float16)
+
+
+def _on(dev: torch.device):
+    """Makes `dev` current for the launches inside."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _one_device(name: str, *ts: torch.Tensor) -> torch.device:
+    _require_cuda(*ts)
+    dev = ts[0].device
+    if any(t.device != dev for t in ts):
+        raise ValueError(f"{name}: all tensors must be on one device")
+    return dev
+
+
+def _check_group(name: str, K: int, group_size: int) -> None:
+    if group_size not in GROUP_SIZES:
+        raise ValueError(f"{name}: group_size {group_size} is not one of {GROUP_SIZES}")
+    if K <= 0 or K % group_size:
+        raise ValueError(f"{name}: the reduction length {K} must be a positive multiple of group_size {group_size}")
+
+
+def quant_int4_groups(w: torch.Tensor, group_size: int = 128, scale_dtype: torch.dtype | None = None):
+    """Rows [R, C] (bf16, fp16 or fp32) -> (q uint8 [R, C / 2], scale [R, C / group_size]).
+
+    scale = absmax / 7 of each group (fp32 quotient, rounded to scale_dtype:
+    w's type, or bf16 for fp32 weights), q = 8 + clamp(w / scale rounded half
+    to even, -8, 7), 8 where the scale is 0. A group that holds a NaN or an
+    infinity, or whose scale scale_dtype cannot hold, gets a NaN scale."""
+    _require_cuda(w)
+    if w.dim() != 2 or w.dtype not in (*_ACT, torch.float32):
+        raise ValueError("quant_int4_groups: expected bf16, fp16 or fp32 weights [R, C]")
+    scale_dtype = scale_dtype or (w.dtype if w.dtype in _ACT else torch.bfloat16)
+    if scale_dtype not in _ACT:
+        raise TypeError(f"quant_int4_groups: scales must be bf16 or fp16, not {scale_dtype}")
+    R, C = w.shape
+    _check_group("quant_int4_groups", C, group_size)
+    w = w.contiguous()
+    q = torch.empty((R, C // 2), dtype=torch.uint8, device=w.device)
+    s = torch.empty((R, C // group_size), dtype=scale_dtype, device=w.device)
+    with _on(w.device):
+        _lib.call("moe_quant_int4_groups", w.data_ptr(), _code(w), R, C, group_size, q.data_ptr(), s.data_ptr(),
+                  _code(s), _stream(w.device))
+    return q, s
+
+
+def dequant_int4_groups(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """(q uint8 [R, C / 2], scale [R, C / group_size]) -> the values [R, C] they
+    stand for, in dtype (the scales' type by default; each product is rounded
+    to it once)."""
+    dev = _one_device("dequant_int4_groups", q, scale)
+    if q.dim() != 2 or q.dtype != torch.uint8 or scale.dim() != 2 or scale.dtype not in _ACT:
+        raise ValueError("dequant_int4_groups: expected q uint8 [R, C / 2] and bf16 or fp16 scales [R, C / group_size]")
+    R, C = q.shape[0], 2 * q.shape[1]
+    if scale.shape[0] != R or scale.shape[1] == 0 or C % scale.shape[1]:
+        raise ValueError(f"dequant_int4_groups: scales {tuple(scale.shape)} do not fit q {tuple(q.shape)}")
+    group_size = C // scale.shape[1]
+    _check_group("dequant_int4_groups", C, group_size)
+    out = torch.empty((R, C), dtype=dtype or scale.dtype, device=dev)
+    if out.dtype not in (*_ACT, torch.float32):
+        raise TypeError(f"dequant_int4_groups: dtype must be bf16, fp16 or fp32, not {out.dtype}")
+    q, scale = q.contiguous(), scale.contiguous()
+    with _on(dev):
+        _lib.call("moe_dequant_int4_groups", q.data_ptr(), scale.data_ptr(), _code(scale), R, C, group_size,
+                  out.data_ptr(), _code(out), _stream(dev))
+    return out
+
+
+def quantize_weights_int4(w13: torch.Tensor, w2: torch.Tensor, group_size: int = 128,
+                          scale_dtype: torch.dtype | None = None):
+    """Load-time weight prep: logical (E, K, N) weights -> 4-bit logical views
+    with K-major storage and their group scales (quant_int4_groups on the
+    K-major rows). Returns (w13_q [E, H / 2, 2I], w2_q [E, I / 2, H],
+    (w13_scale [E, 2I, H / group_size], w2_scale [E, H, I / group_size]))."""
+    def pack(w):
+        wk = kmajor(w)
+        E, N, K = wk.shape
+        q, s = quant_int4_groups(wk.reshape(E * N, K), group_size, scale_dtype)
+        return q.view(E, N, K // 2).transpose(1, 2), s.view(E, N, K // group_size)
+    a, sa = pack(w13)
+    b, sb = pack(w2)
+    return a, b, (sa, sb)
+
+
+def _check_weight(name: str, dtype: torch.dtype, w: torch.Tensor, scale: torch.Tensor, K: int) -> int:
+    """Group size of a 4-bit weight [E, K / 2, N] with scales [E, N, K / g]."""
+    if dtype not in _ACT:
+        raise TypeError(f"{name}: 4-bit weights take bf16 or fp16 activations, not {dtype}")
+    if w.dim() != 3 or w.dtype != torch.uint8 or 2 * w.shape[1] != K:
+        raise ValueError(f"{name}: expected 4-bit weights uint8 [E, K / 2, N] with K = {K}, "
+                         f"got {w.dtype} {tuple(w.shape)}")
+    if scale.dtype != dtype:
+        raise TypeError(f"{name}: the scales must share the activations' type {dtype}, not {scale.dtype}")
+    if scale.dim() != 3 or tuple(scale.shape[:2]) != (w.shape[0], w.shape[2]) or scale.shape[2] == 0 \
+            or K % scale.shape[2]:
+        raise ValueError(f"{name}: scales {tuple(scale.shape)} do not fit weights {tuple(w.shape)} "
+                         "(expected [E, N, K / group_size])")
+    group_size = K // scale.shape[2]
+    _check_group(name, K, group_size)
+    return group_size
+
+
+def _counts(name: str, group_sizes: torch.Tensor, E: int) -> torch.Tensor:
+    if group_sizes.numel() != E:
+        raise ValueError(f"{name}: group_sizes must have E entries")
+    if group_sizes.dtype not in (torch.int32, torch.int64):
+        group_sizes = group_sizes.to(torch.int64)
+    return group_sizes.contiguous()
+
+
+def grouped_matmul_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
+                        group_sizes: torch.Tensor) -> torch.Tensor:
+    """Matrix product grouped by expert, with 4-bit weights: x [T, K] (bf16 or
+    fp16) holds the rows of expert 0, then those of expert 1, and so on;
+    group_sizes [E] says how many each has (any number, zero included; counts
+    past T are cut off). Returns [T, N] in x's type,
+
+        out[r, n] = sum_k x[r, k] * W[e(r), k, n]
+
+    with w uint8 [E, K / 2, N] (K-major storage) and scale [E, N, K / group_size];
+    rows behind the last group are zero. Under torch.compile the call is one
+    operator (torch.ops.mail_b200.grouped_matmul_int4)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.mail_b200.grouped_matmul_int4(x, w, scale, group_sizes)
+    return _grouped_impl(x, w, scale, group_sizes)
+
+
+def _grouped_impl(x, w, scale, group_sizes):
+    name = "grouped_matmul_int4"
+    dev = _one_device(name, x, w, scale, group_sizes)
+    if x.dim() != 2:
+        raise ValueError(f"{name}: expected x [T, K]")
+    T, K = x.shape
+    group_size = _check_weight(name, x.dtype, w, scale, K)
+    E, _, N = w.shape
+    gs = _counts(name, group_sizes, E)
+    x, wk, scale = x.contiguous(), kmajor(w), scale.contiguous()
+    out = torch.empty((T, N), dtype=x.dtype, device=dev)
+    with _on(dev):
+        _lib.call("moe_grouped_matmul_int4", x.data_ptr(), _code(x), T, K, wk.data_ptr(), scale.data_ptr(),
+                  group_size, E, N, gs.data_ptr(), _code(gs), out.data_ptr(), _stream(dev))
+    return out
+
+
+def _layer_weights(x, w13, w2, w13_scale, w2_scale):
+    """(E, H, I, group size, K-major w13, scales, K-major w2, scales), checked."""
+    name = "fused_moe_mlp"
+    if w13_scale is None or w2_scale is None:
+        raise ValueError(f"{name}: 4-bit weights need scales=(w13_scale, w2_scale)")
+    if w2.dtype != torch.uint8:
+        raise TypeError(f"{name}: w13 and w2 must both be 4-bit (uint8)")
+    H = x.shape[1]
+    E, _, two_i = w13.shape
+    group = _check_weight(name, x.dtype, w13, w13_scale, H)
+    if _check_weight(name, x.dtype, w2, w2_scale, two_i // 2) != group:
+        raise ValueError(f"{name}: w13 and w2 must share a group size")
+    return E, H, two_i // 2, group, kmajor(w13), w13_scale.contiguous(), kmajor(w2), w2_scale.contiguous()
+
+
+def fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
+    """The top-k form of fused_moe_mlp with 4-bit weights (shapes checked by
+    the caller)."""
+    E, H, inter, group, a, sa, b, sb = _layer_weights(x, w13, w2, w13_scale, w2_scale)
+    dev = _one_device("fused_moe_mlp", x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale)
+    x = x.contiguous()
+    wts = topk_weights.to(torch.float32).contiguous()
+    ids = topk_ids.to(torch.int32).contiguous()
+    T, k = ids.shape
+    y = torch.empty((T, H), dtype=x.dtype, device=dev)
+    ws = _workspace(_lib.query("moe_fused_experts_int4_workspace_size", T, H, inter, E, k), dev)
+    with _on(dev):
+        _lib.call("moe_fused_experts_int4", x.data_ptr(), _code(x), T, H, a.data_ptr(), sa.data_ptr(), b.data_ptr(),
+                  sb.data_ptr(), group, E, inter, wts.data_ptr(), ids.data_ptr(), k, y.data_ptr(), ws.data_ptr(),
+                  ws.numel(), _stream(dev))
+    return y
+
+
+def fused_mlp(x, w13, w2, group_sizes, w13_scale, w2_scale):
+    """The pre-routed form of fused_moe_mlp with 4-bit weights."""
+    _require_cuda(x, w13, w2, group_sizes)
+    _check_shapes(x, w13, w2)
+    E, H, inter, group, a, sa, b, sb = _layer_weights(x, w13, w2, w13_scale, w2_scale)
+    dev = _one_device("fused_moe_mlp", x, w13, w2, group_sizes, w13_scale, w2_scale)
+    x = x.contiguous()
+    gs = _counts("fused_moe_mlp", group_sizes, E)
+    T = x.shape[0]
+    out = torch.empty((T, H), dtype=x.dtype, device=dev)
+    ws = _workspace(_lib.query("moe_fused_mlp_int4_workspace_size", T, inter, E), dev)
+    with _on(dev):
+        _lib.call("moe_fused_mlp_int4", x.data_ptr(), _code(x), T, H, a.data_ptr(), sa.data_ptr(), b.data_ptr(),
+                  sb.data_ptr(), group, E, inter, gs.data_ptr(), _code(gs), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                  _stream(dev))
+    return out
+
+
+@torch.library.custom_op("mail_b200::fused_moe_mlp_int4", mutates_args=())
+def _op_prerouted(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, group_sizes: torch.Tensor,
+                  w13_scale: torch.Tensor, w2_scale: torch.Tensor) -> torch.Tensor:
+    return fused_mlp(x, w13, w2, group_sizes, w13_scale, w2_scale)
+
+
+@_op_prerouted.register_fake
+def _(x, w13, w2, group_sizes, w13_scale, w2_scale):
+    T, H, E, _ = _check_shapes(x, w13, w2)
+    if group_sizes.numel() != E:
+        raise ValueError("fused_moe_mlp: group_sizes must have E entries")
+    return x.new_empty((T, H))
+
+
+@torch.library.custom_op("mail_b200::grouped_matmul_int4", mutates_args=())
+def _op_grouped(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, group_sizes: torch.Tensor) -> torch.Tensor:
+    return _grouped_impl(x, w, scale, group_sizes)
+
+
+@_op_grouped.register_fake
+def _(x, w, scale, group_sizes):
+    _check_weight("grouped_matmul_int4", x.dtype, w, scale, x.shape[1])
+    return x.new_empty((x.shape[0], w.shape[2]))

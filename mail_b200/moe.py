@@ -85,7 +85,8 @@ def weights_from_linear(w13_linear: torch.Tensor, w2_linear: torch.Tensor):
     return w13_linear.transpose(1, 2), w2_linear.transpose(1, 2)
 
 
-def weights_from_checkpoint(gate_proj, up_proj, down_proj, device=None, dtype=None, quantize: bool = False):
+def weights_from_checkpoint(gate_proj, up_proj, down_proj, device=None, dtype=None, quantize: bool | str = False,
+                            group_size: int = 128):
     """Per-expert checkpoint tensors -> the op's weight storage, once at load.
 
     gate_proj[e] and up_proj[e] are the HF `experts.{e}.gate_proj.weight` /
@@ -99,9 +100,12 @@ def weights_from_checkpoint(gate_proj, up_proj, down_proj, device=None, dtype=No
     layout the kernels' TMA reads) on `device` (default: the tensors' own),
     cast to `dtype` if given — no concatenated or stacked intermediate.
 
-    quantize=True (CUDA device) converts to w8a8 weights with per-output-
-    channel scales (quantize_weights_int8) and returns (w13_q, w2_q, scales);
-    otherwise (w13, w2)."""
+    quantize=True or "int8" (CUDA device) converts to w8a8 weights with
+    per-output-channel scales (quantize_weights_int8), "int4" to 4-bit weights
+    with scales for groups of group_size (quantize_weights_int4); both return
+    (w13_q, w2_q, scales); otherwise (w13, w2)."""
+    if quantize not in (False, True, "int8", "int4"):
+        raise ValueError(f"weights_from_checkpoint: quantize must be a bool, 'int8' or 'int4', not {quantize!r}")
     E = len(gate_proj)
     if len(up_proj) != E or len(down_proj) != E or E == 0:
         raise ValueError("weights_from_checkpoint: gate_proj, up_proj and down_proj need one entry per expert")
@@ -124,7 +128,7 @@ def weights_from_checkpoint(gate_proj, up_proj, down_proj, device=None, dtype=No
     if not quantize:
         return w13l, w2l
     _require_cuda(w13l)
-    return quantize_weights_int8(w13l, w2l)
+    return int4.quantize_weights_int4(w13l, w2l, group_size) if quantize == "int4" else quantize_weights_int8(w13l, w2l)
 
 
 # ---------------------------------------------------------------------------
@@ -246,7 +250,8 @@ def _check_shapes(x, w13, w2):
     T, H = x.shape
     E, Hw, two_i = w13.shape
     inter = two_i // 2
-    if Hw != H or two_i != 2 * inter or tuple(w2.shape) != (E, inter, H):
+    per = 2 if w13.dtype == torch.uint8 else 1  # 4-bit weights: two along K in a byte
+    if Hw * per != H or two_i != 2 * inter or tuple(w2.shape) != (E, inter // per, H) or inter % per:
         raise ValueError(f"fused_moe_mlp: shape mismatch x{tuple(x.shape)} w13{tuple(w13.shape)} "
                          f"w2{tuple(w2.shape)} (expected w13 [E, H, 2I], w2 [E, I, H])")
     return T, H, E, inter
@@ -293,13 +298,15 @@ def _topk_impl(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
     """moe_fused_experts: align -> GEMMs -> weighted combine."""
     _require_cuda(x, w13, w2, topk_weights, topk_ids)
     T, H, E, inter = _check_shapes(x, w13, w2)
+    if topk_weights.shape != topk_ids.shape or topk_ids.dim() != 2 or topk_ids.shape[0] != T:
+        raise ValueError("fused_moe_mlp: topk_weights/topk_ids must both be [T, k]")
+    if w13.dtype == torch.uint8:
+        return int4.fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale)
     x = x.contiguous()
     w13k, w2k = kmajor(w13), kmajor(w2)
     dev = x.device
     topk_weights = topk_weights.to(torch.float32).contiguous()
     ids = topk_ids.to(torch.int32).contiguous()
-    if topk_weights.shape != ids.shape or ids.dim() != 2 or ids.shape[0] != T:
-        raise ValueError("fused_moe_mlp: topk_weights/topk_ids must both be [T, k]")
     k = ids.shape[1]
     w_code, s13, s2 = _weight_scales(x, w13, w2, w13_scale, w2_scale, E, H, inter)
     y = torch.empty((T, H), dtype=x.dtype, device=dev)
@@ -360,18 +367,28 @@ def fused_moe_mlp(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, group_si
     (by at most one bf16 rounding step); larger outputs use a deterministic
     row-store combine.
 
+    Both forms take 4-bit weights with group scales (quantize_weights_int4):
+    uint8 w13 [E, H / 2, 2I] and w2 [E, I / 2, H] with scales=(w13_scale
+    [E, 2I, H / group_size], w2_scale [E, H, I / group_size]) in x's type
+    (bf16 or fp16). Their combine adds a token's rows in slot order, so
+    results do not differ from run to run.
+
     Under torch.compile the call is one operator (torch.ops.mail_b200.
-    fused_moe_mlp / fused_experts); eager calls go straight to the library.
+    fused_moe_mlp / fused_moe_mlp_int4 / fused_experts); eager calls go straight to the library.
     BLOCK_* are accepted for signature compatibility; the sm_100a kernels use
     fixed 128 x 256 tiles and results do not depend on them.
     """
     del BLOCK_M, BLOCK_N, BLOCK_N2, BLOCK_K
     compiling = torch.compiler.is_compiling()
+    s13, s2 = scales if scales is not None else (None, None)
     if topk_ids is None:
+        if w13.dtype == torch.uint8:
+            if compiling:
+                return torch.ops.mail_b200.fused_moe_mlp_int4(x, w13, w2, group_sizes_or_topk_weights, s13, s2)
+            return int4.fused_mlp(x, w13, w2, group_sizes_or_topk_weights, s13, s2)
         if compiling:
             return torch.ops.mail_b200.fused_moe_mlp(x, w13, w2, group_sizes_or_topk_weights)
         return _prerouted_impl(x, w13, w2, group_sizes_or_topk_weights)
-    s13, s2 = scales if scales is not None else (None, None)
     if compiling:
         return torch.ops.mail_b200.fused_experts(x, w13, w2, group_sizes_or_topk_weights, topk_ids, s13, s2)
     return _topk_impl(x, w13, w2, group_sizes_or_topk_weights, topk_ids, s13, s2)
@@ -392,6 +409,9 @@ def _from_logits_impl(x, w13, w2, router_logits, top_k, scoring, renormalize, w1
     """moe_fused_experts_from_logits: router -> align -> GEMMs -> combine."""
     _require_cuda(x, w13, w2, router_logits)
     T, H, E, inter = _check_logits(x, w13, w2, router_logits, top_k, scoring)
+    if w13.dtype == torch.uint8:
+        ids, wts = route_topk(router_logits, top_k, scoring, renormalize)
+        return int4.fused_experts(x, w13, w2, wts, ids, w13_scale, w2_scale), wts, ids
     lg = router_logits.contiguous()
     x = x.contiguous()
     w13k, w2k = kmajor(w13), kmajor(w2)
@@ -485,7 +505,7 @@ class CapturedMoeMLP:
     def __init__(self, w13: torch.Tensor, w2: torch.Tensor, num_tokens: int, top_k: int, dtype=torch.bfloat16,
                  scales=None, inputs=None):
         dev = w13.device
-        H = w13.shape[1]
+        H = w13.shape[1] * (2 if w13.dtype == torch.uint8 else 1)
         if inputs is None:
             self.x = torch.zeros((num_tokens, H), dtype=dtype, device=dev)
             self.w = torch.zeros((num_tokens, top_k), dtype=torch.float32, device=dev)
@@ -523,3 +543,6 @@ def device_error(device=None) -> int:
     code = ctypes.c_int(0)
     _lib.call("moe_get_device_error", ctypes.addressof(code), _stream(dev))
     return code.value
+
+
+from . import int4  # noqa: E402  (the 4-bit forms, which build on the helpers above)
