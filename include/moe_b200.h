@@ -135,7 +135,12 @@ typedef enum {
                                With 1 a batch whose gate_up work is split along K runs as clusters of the
                                split CTAs, which add their partial sums through distributed shared memory
                                (when every cluster of the grid can be resident at once); 2: the same kernel
-                               without clusters, partial sums through global memory */
+                               without clusters, partial sums through global memory */,
+  MOE_OPT_INT4_GEMM = 10      /* products with 4-bit weights: 1: always as tensor-core tiles (tcgen05) of decoded
+                               weights; 0: always by the row kernels, which keep the weights in registers;
+                               2 (default): tiles when the rows average more than a few per expert. The
+                               workspace of moe_fused_experts_int4 depends on it: size it under the same
+                               setting */
 } moe_option_t;
 MOE_API int moe_set_option(int option, int value);
 /* Current value of an option, or -1 for an unknown option. */

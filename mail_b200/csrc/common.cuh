@@ -254,6 +254,14 @@ int decode_fused(const void* x, int dtype, int64_t T, int64_t H, const void* w13
                  const float* topk_weights, const int32_t* topk_ids, int k, void* y, void* workspace,
                  size_t workspace_bytes, cudaStream_t st, const DecodeRouting* route = nullptr);
 
+// Products grouped by expert with 4-bit weights on the tensor cores
+// (moe_gemm_int4.cuh): counts [E] rows of x in a row for each expert; swiglu: w
+// holds n_out gate and n_out up rows. Rows that no expert has are zeroed.
+bool int4_gemm_fits(int64_t rows, int64_t n_out, int64_t w_rows, int E);
+int int4_gemm(const void* x, int dtype, int64_t rows, int64_t k, const uint8_t* w, const void* scale, int group, int E,
+              int64_t n_out, bool swiglu, const void* counts, int counts_is64, void* out, bool out_f32,
+              cudaStream_t st);
+
 // Token-order scatter of the routed rows (+ per-token int8 quantisation):
 // dst[slot_pos[t * k + j]] = row t of src, each row read once (moe_rows.cu).
 bool scatter_rows_fits(int64_t cols);

@@ -871,6 +871,9 @@ std::atomic<int> g_gemm_swap{2};
 // that receives any.
 constexpr int64_t kSwapRowsPerExpert = 64;
 
+// Products with 4-bit weights on the tensor cores (MOE_OPT_INT4_GEMM).
+std::atomic<int> g_int4_gemm{2};
+
 bool use_pair(int64_t max_tiles, int E, int64_t n_tiles) {
   const int v = g_gemm_cta_pair.load();
   if (v == 2) return max_tiles >= 4 * (int64_t)E || max_tiles * n_tiles < num_sms();
@@ -953,6 +956,7 @@ int check_gemm_common(const char* fn, int dtype, int64_t k, int E, const int32_t
 
 #include "moe_gemm_swap.cuh"
 #include "moe_decode.cuh"
+#include "moe_gemm_int4.cuh"
 
 using namespace moe;
 
@@ -1304,6 +1308,11 @@ extern "C" int moe_set_option(int option, int value) {
     g_gemm_swap.store(value);
     return MOE_OK;
   }
+  if (option == MOE_OPT_INT4_GEMM) {
+    MOE_CHECK_ARG(value >= 0 && value <= 2, "moe_set_option: INT4_GEMM takes 0, 1 or 2");
+    g_int4_gemm.store(value);
+    return MOE_OK;
+  }
   return set_error(MOE_ERR_INVALID_ARG, "moe_set_option: unknown option %d", option);
 }
 
@@ -1317,6 +1326,7 @@ extern "C" int moe_get_option(int option) {
   if (option == MOE_OPT_PDL) return g_pdl.load();
   if (option == MOE_OPT_KERNEL_CLOCKS) return g_kernel_clocks_on.load();
   if (option == MOE_OPT_GEMM_SWAP_AB) return g_gemm_swap.load();
+  if (option == MOE_OPT_INT4_GEMM) return g_int4_gemm.load();
   return -1;
 }
 

@@ -423,6 +423,14 @@ int launch_rows_group(MvParams p, int64_t rows, cudaStream_t st) {
   return launch_rows_nt<T, GROUP, 4, SWIGLU>(p, st);
 }
 
+// Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM).
+constexpr int64_t kRowsPerExpert = 16;
+bool use_gemm(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
+  const int opt = moe_get_option(MOE_OPT_INT4_GEMM);
+  if (opt == 0 || rows == 0 || !int4_gemm_fits(rows, n_out, w_rows, E)) return false;
+  return opt == 1 || rows > kRowsPerExpert * std::min<int64_t>(E, rows);
+}
+
 // rows: how many rows there are in all
 template <bool SWIGLU>
 int launch_rows(const MvParams& p, int dtype, int group, int64_t rows, cudaStream_t st) {
@@ -436,8 +444,17 @@ int launch_rows(const MvParams& p, int dtype, int group, int64_t rows, cudaStrea
   return launch_rows_group<__half, 32, SWIGLU>(p, rows, st);
 }
 
+// A product over consecutive rows of each expert, whichever way.
+template <bool SWIGLU>
+int launch_grouped(const MvParams& p, int dtype, int group, bool gemm, cudaStream_t st) {
+  if (!gemm) return launch_rows<SWIGLU>(p, dtype, group, p.total_rows, st);
+  return int4_gemm(p.x, dtype, p.total_rows, p.K, p.w, p.scale, group, p.E, p.n_out, SWIGLU, p.counts, p.counts_is64,
+                   p.out, p.out_f32 != 0, st);
+}
+
 struct LayerWs {
-  size_t h, o, align, sorted, slot_pos, gs, poff, table, align_bytes, bytes;
+  size_t xp, h, o, align, sorted, slot_pos, gs, poff, table, align_bytes, bytes;
+  bool gemm;    // tensor-core tiles
   bool direct;  // the top-k ids are read by the product kernels themselves
 };
 LayerWs layer_ws(int64_t T, int64_t H, int64_t I, int E, int k) {
@@ -449,7 +466,9 @@ LayerWs layer_ws(int64_t T, int64_t H, int64_t I, int E, int k) {
     off = align_up(off + bytes, 256);
     return o;
   };
-  w.direct = S <= kMaxSlots;
+  w.gemm = use_gemm(S, std::max(H, I), std::max(H, 2 * I), E);
+  w.direct = !w.gemm && S <= kMaxSlots;
+  w.xp = take(w.gemm ? (size_t)S * H * 2 : 0);
   w.h = take((size_t)S * I * 2);
   w.o = take((size_t)S * H * sizeof(float));
   if (!w.direct) {
@@ -553,7 +572,7 @@ extern "C" int moe_grouped_matmul_int4(const void* x, int dtype, int64_t num_row
   p.counts_is64 = gs_dtype == MOE_I64;
   p.total_rows = num_rows;
   p.x_div = 1;
-  return launch_rows<false>(p, dtype, group_size, num_rows, as_stream(stream));
+  return launch_grouped<false>(p, dtype, group_size, use_gemm(num_rows, n, n, num_experts), as_stream(stream));
 }
 
 extern "C" size_t moe_fused_experts_int4_workspace_size(int64_t num_tokens, int64_t hidden, int64_t inter,
@@ -598,13 +617,25 @@ extern "C" int moe_fused_experts_int4(const void* x, int dtype, int64_t num_toke
     p.row_map = sorted;
   }
   p.x = x;
+  if (w.gemm) {
+    // each token's row to its place in every expert's run of rows
+    const int32_t* slot_pos = reinterpret_cast<const int32_t*>(ws + w.slot_pos);
+    if (scatter_rows_fits(hidden))
+      MOE_TRY(scatter_rows(x, dtype, hidden, slot_pos, top_k, num_tokens, ws + w.xp, dtype, nullptr, st));
+    else
+      MOE_TRY(gather_rows(x, dtype, hidden, p.row_map, top_k, S,
+                          reinterpret_cast<const int32_t*>(ws + w.table) + 1, ws + w.xp, dtype, nullptr, false, stream));
+    p.x = ws + w.xp;
+    p.row_map = nullptr;
+    p.x_div = 1;
+  }
   p.w = w13;
   p.scale = w13_scale;
   p.out = ws + w.h;
   p.K = hidden;
   p.n_out = (int)inter;
   p.w_rows = (int)(2 * inter);
-  MOE_TRY(launch_rows<true>(p, dtype, group_size, S, st));
+  MOE_TRY(launch_grouped<true>(p, dtype, group_size, w.gemm, st));
   p.x = ws + w.h;
   p.w = w2;
   p.scale = w2_scale;
@@ -614,7 +645,7 @@ extern "C" int moe_fused_experts_int4(const void* x, int dtype, int64_t num_toke
   p.n_out = p.w_rows = (int)hidden;
   p.row_map = nullptr;
   p.x_div = 1;
-  MOE_TRY(launch_rows<false>(p, dtype, group_size, S, st));
+  MOE_TRY(launch_grouped<false>(p, dtype, group_size, w.gemm, st));
   const int64_t h8 = hidden / 8;
   const int32_t* slot_row = w.direct ? nullptr : reinterpret_cast<const int32_t*>(ws + w.slot_pos);
   const float* o = reinterpret_cast<const float*>(ws + w.o);
@@ -664,12 +695,13 @@ extern "C" int moe_fused_mlp_int4(const void* x, int dtype, int64_t num_tokens, 
   p.K = hidden;
   p.n_out = (int)inter;
   p.w_rows = (int)(2 * inter);
-  MOE_TRY(launch_rows<true>(p, dtype, group_size, num_tokens, st));
+  const bool gemm = use_gemm(num_tokens, std::max(hidden, inter), std::max(hidden, 2 * inter), num_experts);
+  MOE_TRY(launch_grouped<true>(p, dtype, group_size, gemm, st));
   p.x = workspace;
   p.w = w2;
   p.scale = w2_scale;
   p.out = out;
   p.K = inter;
   p.n_out = p.w_rows = (int)hidden;
-  return launch_rows<false>(p, dtype, group_size, num_tokens, st);
+  return launch_grouped<false>(p, dtype, group_size, gemm, st);
 }

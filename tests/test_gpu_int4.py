@@ -22,6 +22,17 @@ BF, HF = torch.bfloat16, torch.float16
 DEV = "cuda"
 
 
+@pytest.fixture(params=["rows", "tiles"])
+def kernel(request):
+    """Each test with the row kernels and with the tensor-core tiles."""
+    lib = _lib.load()
+    before = lib.moe_get_option(_lib.OPT_INT4_GEMM)
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, int(request.param == "tiles")) == 0
+    yield request.param
+    assert mb.device_error() == 0
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, before) == 0
+
+
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
@@ -178,7 +189,7 @@ GROUPED = [
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("K,N,group,sizes", GROUPED)
-def test_grouped_matmul_exact(dtype, K, N, group, sizes):
+def test_grouped_matmul_exact(dtype, K, N, group, sizes, kernel):
     E, T = len(sizes), sum(sizes)
     w, s, wide = weights(E, N, K, group, dtype, K + N, exact=True)
     x = small_ints((T, K), dtype, T)
@@ -190,7 +201,7 @@ def test_grouped_matmul_exact(dtype, K, N, group, sizes):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("K,N,group,sizes", GROUPED)
-def test_grouped_matmul_random(dtype, K, N, group, sizes):
+def test_grouped_matmul_random(dtype, K, N, group, sizes, kernel):
     E, T = len(sizes), sum(sizes)
     w, s, wide = weights(E, N, K, group, dtype, K)
     x = torch.randn((T, K), device=DEV, generator=gen(N)).to(dtype)
@@ -200,7 +211,7 @@ def test_grouped_matmul_random(dtype, K, N, group, sizes):
 
 
 @pytest.mark.parametrize("sizes", [[3, 0, 2], [0, 0, 0], [4, 4, 40], [-3, 5, 0], [12, 0, 0]])
-def test_grouped_matmul_sizes_that_do_not_add_up(sizes):
+def test_grouped_matmul_sizes_that_do_not_add_up(sizes, kernel):
     """Rows behind the last group are zero; counts past the rows are cut off;
     negative counts are empty groups."""
     T, K, N = 12, 128, 50
@@ -214,7 +225,7 @@ def test_grouped_matmul_sizes_that_do_not_add_up(sizes):
     assert out.shape == (0, N)
 
 
-def test_grouped_matmul_many_experts_and_offsets():
+def test_grouped_matmul_many_experts_and_offsets(kernel):
     E, K, N = 1024, 64, 24
     sizes = torch.randint(0, 4, (E,), device=DEV, generator=gen(2))
     w, s, wide = weights(E, N, K, 32, HF, 1, exact=True)
@@ -223,7 +234,7 @@ def test_grouped_matmul_many_experts_and_offsets():
     assert torch.equal(mb.grouped_matmul_int4(x, w, s, sizes), ref.to(HF))
 
 
-def test_grouped_matmul_weights_past_32_bit_offsets():
+def test_grouped_matmul_weights_past_32_bit_offsets(kernel):
     """The last expert's weights lie behind 2^32 nibbles."""
     E, K, N = 9, 7168, 65536 + 8192
     assert E * K * N > 2 ** 32
@@ -239,7 +250,7 @@ def test_grouped_matmul_weights_past_32_bit_offsets():
     assert torch.equal(mb.grouped_matmul_int4(x, packed.transpose(1, 2), s, sizes), ref.to(BF))
 
 
-def test_grouped_matmul_strided_inputs_and_other_layouts():
+def test_grouped_matmul_strided_inputs_and_other_layouts(kernel):
     w, s, wide = weights(3, 48, 256, 64, BF, 5, exact=True)
     sizes = torch.tensor([2, 0, 3], device=DEV)
     big = small_ints((10, 512), BF, 3)
@@ -253,7 +264,7 @@ def test_grouped_matmul_strided_inputs_and_other_layouts():
     assert torch.equal(mb.grouped_matmul_int4(x, w, s, every), ref.to(BF))
 
 
-def test_grouped_matmul_keeps_nan_and_inf_to_their_rows():
+def test_grouped_matmul_keeps_nan_and_inf_to_their_rows(kernel):
     w, s, wide = weights(2, 64, 256, 128, BF, 5, exact=True)
     x = small_ints((20, 256), BF, 3)
     ref, _ = grouped_ref(x, wide, [9, 11])
@@ -285,7 +296,7 @@ LAYER = [
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("T,E,k,H,I,group", LAYER)
-def test_layer(dtype, T, E, k, H, I, group):
+def test_layer(dtype, T, E, k, H, I, group, kernel):
     w13, s13, wide13 = weights(E, 2 * I, H, group, dtype, 1)
     w2, s2, wide2 = weights(E, H, I, group, dtype, 2)
     x = torch.randn((T, H), device=DEV, generator=gen(3)).to(dtype)
@@ -299,7 +310,7 @@ def test_layer(dtype, T, E, k, H, I, group):
 
 
 @pytest.mark.parametrize("T", [3, 40, 700])
-def test_layer_slots_that_name_no_expert(T):
+def test_layer_slots_that_name_no_expert(T, kernel):
     """Ids outside [0, E) add nothing, a token without any gives zeros, an
     expert named twice by one token counts twice."""
     E, k, H, I = 6, 4, 256, 128
@@ -317,7 +328,7 @@ def test_layer_slots_that_name_no_expert(T):
 
 
 @pytest.mark.parametrize("T", [2, 130, 600])
-def test_layer_from_logits_matches_router_and_layer(T):
+def test_layer_from_logits_matches_router_and_layer(T, kernel):
     E, k, H, I = 16, 4, 256, 128
     w13, s13, _ = weights(E, 2 * I, H, 64, BF, 1)
     w2, s2, _ = weights(E, H, I, 64, BF, 2)
@@ -330,7 +341,7 @@ def test_layer_from_logits_matches_router_and_layer(T):
 
 
 @pytest.mark.parametrize("sizes", [[1, 0, 0], [3, 9, 0], [40, 0, 77], [200, 300, 140]])
-def test_pre_routed_layer(sizes):
+def test_pre_routed_layer(sizes, kernel):
     E, H, I, dtype = 3, 256, 192, HF
     w13, s13, wide13 = weights(E, 2 * I, H, 64, dtype, 1)
     w2, s2, wide2 = weights(E, H, I, 64, dtype, 2)
@@ -344,7 +355,7 @@ def test_pre_routed_layer(sizes):
     assert_within(out, ref, bound, dtype)
 
 
-def test_quantise_then_serve():
+def test_quantise_then_serve(kernel):
     """A checkpoint's weights quantised, then prefill, decode through a
     captured graph and the grouped product on the same weights."""
     E, H, I, k = 8, 512, 256, 2
@@ -375,7 +386,7 @@ def test_quantise_then_serve():
         assert torch.equal(cap(x2, wts2, ids2), mb.fused_moe_mlp(x2, w13, w2, wts2, ids2, scales=scales))
 
 
-def test_two_captured_graphs_do_not_share_state():
+def test_two_captured_graphs_do_not_share_state(kernel):
     E, H, I, k = 8, 256, 128, 2
     w13, s13, _ = weights(E, 2 * I, H, 128, BF, 1)
     w2, s2, _ = weights(E, H, I, 128, BF, 2)
@@ -396,7 +407,7 @@ def test_two_captured_graphs_do_not_share_state():
     assert torch.equal(caps[0].y, want[0]) and torch.equal(caps[1].y, want[1])
 
 
-def test_calls_on_several_streams_at_once():
+def test_calls_on_several_streams_at_once(kernel):
     E, H, I, k = 8, 512, 256, 2
     w13, s13, _ = weights(E, 2 * I, H, 128, BF, 1)
     w2, s2, _ = weights(E, H, I, 128, BF, 2)
@@ -415,7 +426,7 @@ def test_calls_on_several_streams_at_once():
         assert torch.equal(y, want[i % 3])
 
 
-def test_torch_op_takes_4_bit_weights():
+def test_torch_op_takes_4_bit_weights(kernel):
     E, H, I, k, T = 4, 256, 128, 2, 6
     w13, s13, _ = weights(E, 2 * I, H, 128, BF, 1)
     w2, s2, _ = weights(E, H, I, 128, BF, 2)
@@ -450,7 +461,7 @@ def test_refusals_on_the_device():
         mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2[:, 1:]))
     with pytest.raises(ValueError, match="share a group size"):
         mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2.repeat_interleave(2, dim=2)))
-    with pytest.raises(ValueError, match="one device"):
+    with pytest.raises(ValueError, match="CUDA tensors only"):
         mb.grouped_matmul_int4(x, w13, s13, torch.tensor([1, 2, 0, 3], device=DEV).cpu().pin_memory())
     with pytest.raises(TypeError, match="unsupported dtype"):
         mb.fused_expert_rows(x, w13, w2, ids[:, 0], scales=(s13, s2))
