@@ -8,18 +8,19 @@
 // The 128 weight rows of a feature tile are the MMA's M operand and the
 // expert's rows (up to 256, evenly split over its tiles, rounded up to 16) its
 // N operand, so an expert with few rows costs few MMA columns. The tensor
-// cores take 16-bit operands: eight warps turn the 4-bit words into
+// cores take 16-bit operands: eight or twelve warps turn the 4-bit words into
 // (q - 8) s in shared memory while earlier blocks multiply. A weight is
 // rounded to the activations' type there, by at most half a step: scaling
 // after the product instead would read the accumulator once for every group.
 //
-// Roles (480 threads, one CTA per SM, persistent):
-//   warp 0        rows of x: TMA, 64 k by up to 256 rows a block
-//   warp 1        TMEM, single-thread MMA issue into one of two accumulators
+// Roles (one CTA per SM, persistent):
+//   warp 0        rows of x: TMA, 64 k by up to 256 rows a block, one or two
+//                 boxes whose heights are powers of two
+//   warp 1        TMEM, MMA issue into one of two accumulators
 //   warp 2        4-bit words: TMA, 128 k by 128 weight rows a block
 //   warps 3..6    epilogue
-//   warps 7..14   decoding; warps 7..10 the first 64 k of each block of 128,
-//                 warps 11..14 the second, a thread to a weight row
+//   warps 7..     decoding: two or three sets of four warps take the blocks of
+//                 words in turn, a thread to a weight row
 // With SWIGLU a tile's rows alternate between 16 gate rows and the 16 up rows
 // that go with them, so gate and up of a feature sit sixteen TMEM lanes apart
 // in one warp, and a shuffle for every two tokens brings them together.
@@ -28,17 +29,46 @@
 namespace moe {
 namespace {
 
-constexpr int Q4_THREADS = 480;
+constexpr int Q4_FIRST = 7;              // first decoding warp
+constexpr int Q4_MAX_SETS = 3;           // sets of four decoding warps
+constexpr int Q4_THREADS = 32 * (Q4_FIRST + 4 * Q4_MAX_SETS);
 constexpr int Q4_FEAT = 128;             // weight rows of a tile (UMMA M)
-constexpr int Q4_ROWS = 256;             // rows of x of a tile at most (UMMA N)
-constexpr int Q4_BOX = 32;               // rows of x in a TMA box
 constexpr int Q4_KB = 64;                // k of an MMA block (128 bytes of 16-bit type)
 constexpr int Q4_RAW_ROW = 64;           // bytes of 4-bit words in a block of 128 k
 constexpr uint32_t Q4_RAW_BYTES = Q4_FEAT * Q4_RAW_ROW;
 constexpr uint32_t Q4_A_BYTES = Q4_FEAT * ROW_BYTES;
-constexpr uint32_t Q4_X_BYTES = Q4_ROWS * ROW_BYTES;
-constexpr int Q4_SR = 5, Q4_SA = 3, Q4_SX = 4;  // stages: words, decoded weights, rows of x
-constexpr int Q4_AHEAD = 4;              // blocks of 128 k between a scale's load and its use
+constexpr int Q4_MAX_STAGES = 6, Q4_MAX_RAW = 9;
+constexpr int Q4_BOXES = 5;              // boxes of 16, 32, 64, 128 and 256 rows of x
+
+// Rows of x of a tile and pipeline stages. Wide tiles for many rows an expert;
+// narrow ones, with more stages, where the launch is bound by the weights.
+//
+// A wait on a barrier's parity cannot tell use u of a stage from use u - 2, so
+// no set may come to a use before use u - 2 is over for certain. A set that
+// has filled a stage has seen the stage's last use freed, and stages are freed
+// in order; from the last stage of its last block to the first of its next lie
+// at most 2 sets - 1 stages, so sets <= stages / 2 keeps it within one round.
+// Words come in any order: raw is a multiple of sets, so the use before the
+// one that a set waits for was its own.
+struct Int4Shape {
+  int nmax;    // rows of x of a tile at most (UMMA N, at most 256)
+  int stages;  // blocks of decoded weights and rows of x
+  int raw;     // blocks of words
+  int sets;    // sets of decoding warps
+};
+constexpr bool shape_ok(const Int4Shape& s) {
+  return s.sets <= Q4_MAX_SETS && s.stages <= Q4_MAX_STAGES && s.raw <= Q4_MAX_RAW && 2 * s.nmax <= TMEM_COLS &&
+         2 * s.sets <= s.stages && s.raw % s.sets == 0;
+}
+constexpr Int4Shape kInt4Wide{256, 4, 4, 2}, kInt4WideManyExperts{256, 4, 2, 2}, kInt4Narrow{64, 6, 9, 3};
+static_assert(shape_ok(kInt4Wide) && shape_ok(kInt4WideManyExperts) && shape_ok(kInt4Narrow), "ring depths");
+constexpr size_t kMaxSmem = 227 * 1024;
+constexpr int64_t kInt4NarrowRows = 48;  // narrow tiles up to this many rows an expert on average
+
+struct Int4Maps {
+  CUtensorMap w;
+  CUtensorMap x[Q4_BOXES];
+};
 
 struct Int4Params {
   int E;
@@ -53,10 +83,24 @@ struct Int4Params {
   void* out;             // [total_rows, n_out]
   int out_f32;
   uint32_t idesc_m;      // instruction descriptor without the N field
+  Int4Shape shape;
+};
+
+// A place in a ring of barriers.
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int n, int size) {
+    i += n;
+    while (i >= size) {
+      i -= size;
+      phase ^= 1;
+    }
+  }
 };
 
 struct Int4Smem {
-  uint64_t raw_full[Q4_SR], raw_empty[Q4_SR], x_full[Q4_SX], x_empty[Q4_SX], a_full[Q4_SA], a_empty[Q4_SA];
+  uint64_t raw_full[Q4_MAX_RAW], raw_empty[Q4_MAX_RAW], full[Q4_MAX_STAGES], empty[Q4_MAX_STAGES];
   uint64_t tfull[2], tempty[2], drain;
   uint32_t tmem_slot;
   int abort_flag;
@@ -122,33 +166,30 @@ __device__ __forceinline__ uint4 decode_word(uint32_t w, uint32_t s2) {
 }
 
 template <typename T, int GROUP, bool SWIGLU>
-__global__ void __launch_bounds__(Q4_THREADS, 1)
-    int4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                     const Int4Params p) {
+__global__ void __launch_bounds__(Q4_THREADS, 1) int4_gemm_kernel(const __grid_constant__ Int4Maps maps,
+                                                                  const Int4Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stages = p.shape.stages, raws = p.shape.raw, nmax = p.shape.nmax;
+  const uint32_t x_bytes = (uint32_t)nmax * ROW_BYTES;
   uint8_t* sA = smem;
-  uint8_t* sX = sA + Q4_SA * Q4_A_BYTES;
-  uint8_t* sR = sX + Q4_SX * Q4_X_BYTES;
-  Int4Smem& sm = *reinterpret_cast<Int4Smem*>(sR + Q4_SR * Q4_RAW_BYTES);
+  uint8_t* sX = sA + stages * Q4_A_BYTES;
+  uint8_t* sR = sX + stages * x_bytes;
+  Int4Smem& sm = *reinterpret_cast<Int4Smem*>(sR + raws * Q4_RAW_BYTES);
   int32_t* s_off = reinterpret_cast<int32_t*>(&sm + 1);  // [E + 1] first row of each expert
   int32_t* s_cum = s_off + p.E + 1;                      // [E + 1] row tiles before each expert
   volatile int* abort_flag = &sm.abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int E = p.E;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < Q4_SR; ++i) {
+    for (int i = 0; i < raws; ++i) {
       ptx::mbar_init(&sm.raw_full[i], 1);
-      ptx::mbar_init(&sm.raw_empty[i], 8);  // decoding warps
+      ptx::mbar_init(&sm.raw_empty[i], 4);  // the warps of a set
     }
-    for (int i = 0; i < Q4_SX; ++i) {
-      ptx::mbar_init(&sm.x_full[i], 1);
-      ptx::mbar_init(&sm.x_empty[i], 1);
-    }
-    for (int i = 0; i < Q4_SA; ++i) {
-      ptx::mbar_init(&sm.a_full[i], 4);  // the decoding warps of one half
-      ptx::mbar_init(&sm.a_empty[i], 1);
+    for (int i = 0; i < stages; ++i) {
+      ptx::mbar_init(&sm.full[i], 5);  // the rows' copy and the warps of a set
+      ptx::mbar_init(&sm.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&sm.tfull[i], 1);
@@ -157,8 +198,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
     ptx::mbar_init(&sm.drain, 1);
     sm.abort_flag = 0;
     ptx::fence_mbar_init();
-    ptx::prefetch_tmap(&tmap_w);
-    ptx::prefetch_tmap(&tmap_x);
+    ptx::prefetch_tmap(&maps.w);
   }
   pdl_begin();
   if (warp == 2) {
@@ -185,7 +225,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
       run += count(e);
       const int64_t end = min(run, p.total_rows);
       s_off[e] = (int32_t)first;
-      tiles += (int)((end - first + Q4_ROWS - 1) / Q4_ROWS);
+      tiles += (int)((end - first + nmax - 1) / nmax);
     }
     const int64_t all = __shfl_sync(0xffffffffu, incl, 31);
     if (lane == 31) s_off[E] = (int32_t)min(all, p.total_rows);
@@ -199,7 +239,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
     int trun = tincl - tiles;
     for (int e = lo; e < hi; ++e) {
       s_cum[e] = trun;
-      trun += (s_off[e + 1] - s_off[e] + Q4_ROWS - 1) / Q4_ROWS;
+      trun += (s_off[e + 1] - s_off[e] + nmax - 1) / nmax;
     }
     if (lane == 31) s_cum[E] = tincl;
   }
@@ -217,128 +257,127 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ rows of x
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int last_par[Q4_SX];
-#pragma unroll
-      for (int s = 0; s < Q4_SX; ++s) last_par[s] = -1;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
-        const int nbox = (it.rows + Q4_BOX - 1) / Q4_BOX;
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (!ptx::mbar_wait(&sm.x_empty[stage], phase ^ 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          ptx::mbar_arrive_expect_tx(&sm.x_full[stage], nbox * Q4_BOX * ROW_BYTES);
-          for (int b = 0; b < nbox; ++b)
-            ptx::tma_load_2d(sX + stage * Q4_X_BYTES + b * Q4_BOX * ROW_BYTES, &tmap_x, &sm.x_full[stage],
-                             kb * Q4_KB, (int32_t)(it.row + b * Q4_BOX));
-          last_par[stage] = (int)phase;
-          if (++stage == Q4_SX) {
-            stage = 0;
-            phase ^= 1;
-          }
+    Ring ring;
+    int filled = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
+      const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
+      // one box of at least the rows, or two where that would load a third too many
+      const int up = it.rows <= 16 ? 4 : 32 - __clz(it.rows - 1);  // 2^up >= rows
+      const bool two = 4 * it.rows <= 3 << up && up > 5;
+      const int h0 = two ? up - 1 : up;
+      const int rest = it.rows - (1 << h0);
+      const int h1 = rest <= 16 ? 4 : 32 - __clz(rest - 1);
+      const uint32_t bytes = ((1u << h0) + (two ? 1u << h1 : 0u)) * ROW_BYTES;
+      const CUtensorMap* m0 = &maps.x[h0 - 4];
+      const CUtensorMap* m1 = &maps.x[h1 - 4];
+      for (int kb = 0; kb < nkb; ++kb) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.empty[ring.i], ring.phase ^ 1, abort_flag));
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          uint64_t* bar = &sm.full[ring.i];
+          uint8_t* dst = sX + ring.i * x_bytes;
+          ptx::mbar_arrive_expect_tx(bar, bytes);
+          ptx::tma_load_2d(dst, m0, bar, kb * Q4_KB, (int32_t)it.row);
+          if (two) ptx::tma_load_2d(dst + (ROW_BYTES << h0), m1, bar, kb * Q4_KB, (int32_t)it.row + (1 << h0));
         }
-      }
-      if (!ok) {
-        raise_device_error(1);
-        *abort_flag = 1;
-        volatile int never = 0;  // copies in flight land before the CTA exits
-        for (int s = 0; s < Q4_SX; ++s)
-          if (last_par[s] >= 0) ptx::mbar_wait(&sm.x_full[s], (uint32_t)last_par[s], &never);
+        __syncwarp();
+        ring.advance(1, stages);
+        filled = min(filled + 1, stages);
       }
     }
+    if (!ok && lane == 0) {
+      raise_device_error(1);
+      *abort_flag = 1;
+      // copies in flight land before the CTA exits: the stages filled last, newest first
+      volatile int never = 0;
+      for (; filled > 0; --filled) {
+        ring.i = ring.i == 0 ? stages - 1 : ring.i - 1;
+        if (ring.i == stages - 1) ring.phase ^= 1;
+        ptx::mbar_wait(&sm.full[ring.i], ring.phase, &never);
+      }
+    }
+    __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------ 4-bit words
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int last_par[Q4_SR];
-#pragma unroll
-      for (int s = 0; s < Q4_SR; ++s) last_par[s] = -1;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
-        const int wrow = it.e * p.w_rows + it.f * (SWIGLU ? Q4_FEAT / 2 : Q4_FEAT);
-        for (int kb = 0; kb < nraw; ++kb) {
-          if (!ptx::mbar_wait(&sm.raw_empty[stage], phase ^ 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          ptx::mbar_arrive_expect_tx(&sm.raw_full[stage], Q4_RAW_BYTES);
-          uint8_t* dst = sR + stage * Q4_RAW_BYTES;
-          ptx::tma_load_2d(dst, &tmap_w, &sm.raw_full[stage], kb * Q4_RAW_ROW, wrow);
+    Ring ring;
+    int filled = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
+      const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
+      const int wrow = it.e * p.w_rows + it.f * (SWIGLU ? Q4_FEAT / 2 : Q4_FEAT);
+      for (int kb = 0; kb < nraw; ++kb) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.raw_empty[ring.i], ring.phase ^ 1, abort_flag));
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          uint64_t* bar = &sm.raw_full[ring.i];
+          uint8_t* dst = sR + ring.i * Q4_RAW_BYTES;
+          ptx::mbar_arrive_expect_tx(bar, Q4_RAW_BYTES);
+          ptx::tma_load_2d(dst, &maps.w, bar, kb * Q4_RAW_ROW, wrow);
           if constexpr (SWIGLU)
-            ptx::tma_load_2d(dst + Q4_RAW_BYTES / 2, &tmap_w, &sm.raw_full[stage], kb * Q4_RAW_ROW, wrow + p.n_out);
-          last_par[stage] = (int)phase;
-          if (++stage == Q4_SR) {
-            stage = 0;
-            phase ^= 1;
-          }
+            ptx::tma_load_2d(dst + Q4_RAW_BYTES / 2, &maps.w, bar, kb * Q4_RAW_ROW, wrow + p.n_out);
         }
-      }
-      if (!ok) {
-        raise_device_error(1);
-        *abort_flag = 1;
-        volatile int never = 0;
-        for (int s = 0; s < Q4_SR; ++s)
-          if (last_par[s] >= 0) ptx::mbar_wait(&sm.raw_full[s], (uint32_t)last_par[s], &never);
+        __syncwarp();
+        ring.advance(1, raws);
+        filled = min(filled + 1, raws);
       }
     }
+    if (!ok && lane == 0) {
+      raise_device_error(1);
+      *abort_flag = 1;
+      volatile int never = 0;
+      for (; filled > 0; --filled) {
+        ring.i = ring.i == 0 ? raws - 1 : ring.i - 1;
+        if (ring.i == raws - 1) ring.phase ^= 1;
+        ptx::mbar_wait(&sm.raw_full[ring.i], ring.phase, &never);
+      }
+    }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      int xs = 0, as = 0, n = 0;
-      uint32_t xphase = 0, aphase = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < total; item += gridDim.x, ++n) {
-        const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
-        const int buf = n & 1;
-        if (!ptx::mbar_wait(&sm.tempty[buf], ((n >> 1) & 1) ^ 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+    // The whole warp runs the loop and one lane issues: descriptors stay in
+    // uniform registers. Issued from a single-lane branch the four MMAs of a
+    // block took 350 cycles to issue, which bound the launch.
+    Ring ring;
+    int n = 0;
+    bool ok = true;
+    const uint64_t a_desc = ptx::smem_desc_k128(ptx::smem_u32(sA)), x_desc = ptx::smem_desc_k128(ptx::smem_u32(sX));
+    for (int item = blockIdx.x; ok && item < total; item += gridDim.x, ++n) {
+      const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
+      const int buf = n & 1;
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.tempty[buf], ((n >> 1) & 1) ^ 1, abort_flag));
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t idesc = p.idesc_m | ((uint32_t)((it.rows + 15) / 16 * 2) << 17);
+      const uint32_t d = tmem_base + (uint32_t)(buf * nmax);
+      for (int kb = 0; kb < nkb; ++kb) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&sm.full[ring.i], ring.phase, abort_flag));
+        if (!ok) break;
         ptx::tc_fence_after();
-        const uint32_t idesc = p.idesc_m | ((uint32_t)((it.rows + 15) / 16 * 2) << 17);
-        const uint32_t d = tmem_base + (uint32_t)(buf * Q4_ROWS);
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (!ptx::mbar_wait(&sm.x_full[xs], xphase, abort_flag) ||
-              !ptx::mbar_wait(&sm.a_full[as], aphase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          ptx::tc_fence_after();
-          const uint32_t a_addr = ptx::smem_u32(sA + as * Q4_A_BYTES);
-          const uint32_t b_addr = ptx::smem_u32(sX + xs * Q4_X_BYTES);
+        const uint64_t ad = a_desc + (uint64_t)(ring.i * (Q4_A_BYTES >> 4));
+        const uint64_t xd = x_desc + (uint64_t)(ring.i * (x_bytes >> 4));
+        if (ptx::elect_one()) {
 #pragma unroll
           for (int k = 0; k < ROW_BYTES / 32; ++k)
-            ptx::umma<0>(d, ptx::smem_desc_k128(a_addr + k * 32), ptx::smem_desc_k128(b_addr + k * 32), idesc,
-                         (kb > 0 || k > 0) ? 1u : 0u);
-          ptx::umma_commit(&sm.x_empty[xs]);
-          ptx::umma_commit(&sm.a_empty[as]);
-          if (++xs == Q4_SX) {
-            xs = 0;
-            xphase ^= 1;
-          }
-          if (++as == Q4_SA) {
-            as = 0;
-            aphase ^= 1;
-          }
+            ptx::umma<0>(d, ad + 2 * k, xd + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          ptx::umma_commit(&sm.empty[ring.i]);
+          if (kb == nkb - 1) ptx::umma_commit(&sm.tfull[buf]);
         }
-        if (ok) ptx::umma_commit(&sm.tfull[buf]);
+        __syncwarp();
+        ring.advance(1, stages);
       }
-      if (!ok) {
-        raise_device_error(2);
-        *abort_flag = 1;
-      }
+    }
+    if (!ok && lane == 0) {
+      raise_device_error(2);
+      *abort_flag = 1;
+    }
+    if (ptx::elect_one()) {
       ptx::umma_commit(&sm.drain);  // all MMAs complete before TMEM is released
       volatile int never = 0;
       if (!ptx::mbar_wait(&sm.drain, 0, &never)) raise_device_error(4);
     }
-  } else if (warp < 7) {
+    __syncwarp();
+  } else if (warp < Q4_FIRST) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;  // TMEM lanes 32 q .. 32 q + 31
     bool ok = true;
@@ -352,7 +391,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
         break;
       }
       ptx::tc_fence_after();
-      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * Q4_ROWS);
+      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * nmax);
       const int feat = SWIGLU ? it.f * (Q4_FEAT / 2) + q * 16 + (lane & 15) : it.f * Q4_FEAT + q * 32 + lane;
       const bool feat_ok = feat < p.n_out;
       const int64_t base = it.row * p.n_out + feat;
@@ -405,13 +444,29 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ decoding
-    const int half = (warp - 7) >> 2;             // which 64 k of a block of 128
-    const int r = ((warp - 7) & 3) * 32 + lane;   // row of the tile
+    const int set = (warp - Q4_FIRST) >> 2;
+    const int r = ((warp - Q4_FIRST) & 3) * 32 + lane;  // row of the tile
     // its row of the word block (gate rows first, then up rows)
     const int rr = SWIGLU ? ((r & 16) ? Q4_FEAT / 2 : 0) + (r >> 5) * 16 + (r & 15) : r;
-    constexpr int NS = GROUP == 32 ? 2 : 1;       // groups in 64 k
+    constexpr int NS = 128 / GROUP;  // groups of a block of words
     const int groups = p.K / GROUP;
-    auto scale_row = [&](const Int4Item& it) -> const T* {
+    // this set's blocks of words: every sets-th of the run of all blocks
+    struct Walk {
+      int item, kb;
+      __device__ __forceinline__ bool step(int n, int nraw) {  // true: another item
+        kb += n;
+        bool moved = false;
+        while (kb >= nraw) {
+          kb -= nraw;
+          item += gridDim.x;
+          moved = true;
+        }
+        return moved;
+      }
+    };
+    auto scale_row = [&](int item) -> const T* {
+      if (item >= total) return nullptr;
+      const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
       int wr;
       if (SWIGLU)
         wr = min(it.f * (Q4_FEAT / 2) + (r >> 5) * 16 + (r & 15), p.n_out - 1) + ((r & 16) ? p.n_out : 0);
@@ -419,83 +474,74 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
         wr = min(it.f * Q4_FEAT + r, p.n_out - 1);
       return static_cast<const T*>(p.scale) + ((int64_t)it.e * p.w_rows + wr) * groups;
     };
-    // scales of word blocks [b0, b0 + Q4_AHEAD); blocks past K get 0
-    auto load_scales = [&](const T* row, int b0, T (&s)[Q4_AHEAD][NS]) {
+    // scales are read two of this set's blocks ahead; groups past K are 0
+    auto load_scales = [&](const T* row, int kb, T (&s)[NS]) {
 #pragma unroll
-      for (int i = 0; i < Q4_AHEAD; ++i)
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          const int g = GROUP == 128 ? b0 + i : GROUP == 64 ? 2 * (b0 + i) + half : 4 * (b0 + i) + 2 * half + j;
-          s[i][j] = g < groups ? row[g] : u4::Act<T>::from_float(0.f);
-        }
-    };
-    int rs = 0, as = half;  // word stage; the decoded stages of this half's blocks
-    uint32_t rphase = 0, aphase = 0;
-    bool ok = true;
-    T cur[Q4_AHEAD][NS], nxt[Q4_AHEAD][NS];
-    const T* row = nullptr;
-    if ((int)blockIdx.x < total) {
-      row = scale_row(int4_item(blockIdx.x, s_cum, s_off, E, p.nf));
-      load_scales(row, 0, cur);
-    }
-    int blk = half;  // index of this half's next block in the run of all MMA blocks
-    int base_blk = 0;
-    for (int item = blockIdx.x; ok && item < total; item += gridDim.x) {
-      for (int b0 = 0; ok && b0 < nraw; b0 += Q4_AHEAD) {
-        if (b0 + Q4_AHEAD < nraw) {
-          load_scales(row, b0 + Q4_AHEAD, nxt);
-        } else if (item + (int)gridDim.x < total) {
-          row = scale_row(int4_item(item + gridDim.x, s_cum, s_off, E, p.nf));
-          load_scales(row, 0, nxt);
-        }
-#pragma unroll
-        for (int i = 0; i < Q4_AHEAD; ++i) {
-          if (!ok || b0 + i >= nraw) continue;
-          const bool live = 2 * (b0 + i) + half < nkb;  // the last block may have one half
-          bool w_ok = ptx::mbar_wait(&sm.raw_full[rs], rphase, abort_flag);
-          uint4 w[2];
-          if (w_ok) {
-            const uint8_t* src = sR + rs * Q4_RAW_BYTES + rr * Q4_RAW_ROW;
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              w[c] = *reinterpret_cast<const uint4*>(src + (((2 * half + c) ^ ((rr >> 1) & 3)) << 4));
-          }
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&sm.raw_empty[rs]);
-          if (++rs == Q4_SR) {
-            rs = 0;
-            rphase ^= 1;
-          }
-          if (live) {
-            blk = base_blk + 2 * (b0 + i) + half;
-            as = blk % Q4_SA;
-            aphase = (uint32_t)(blk / Q4_SA) & 1u;
-            w_ok = w_ok && ptx::mbar_wait(&sm.a_empty[as], aphase ^ 1, abort_flag);
-            if (w_ok) {
-              uint8_t* dst = sA + as * Q4_A_BYTES + r * ROW_BYTES;
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const T s = cur[i][NS == 2 ? c : 0];
-                const uint32_t s1 = *reinterpret_cast<const uint16_t*>(&s);
-                const uint32_t s2 = s1 | (s1 << 16);
-                const uint32_t ws[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  *reinterpret_cast<uint4*>(dst + (((4 * c + k) ^ (r & 7)) << 4)) = decode_word<T>(ws[k], s2);
-              }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sm.a_full[as]);
-          }
-          ok = __all_sync(0xffffffffu, w_ok);
-        }
-#pragma unroll
-        for (int i = 0; i < Q4_AHEAD; ++i)
-#pragma unroll
-          for (int j = 0; j < NS; ++j) cur[i][j] = nxt[i][j];
+      for (int j = 0; j < NS; ++j) {
+        const int g = kb * NS + j;
+        s[j] = row != nullptr && g < groups ? row[g] : u4::Act<T>::from_float(0.f);
       }
-      base_blk += nkb;
+    };
+    Walk cur{(int)blockIdx.x, 0}, ahead;
+    cur.step(set, nraw);
+    ahead = cur;
+    const int sets = p.shape.sets;
+    T s0[NS], s1[NS], s2[NS];
+    const T* row = scale_row(ahead.item);
+    load_scales(row, ahead.kb, s0);
+    if (ahead.step(sets, nraw)) row = scale_row(ahead.item);
+    load_scales(row, ahead.kb, s1);
+    Ring raw, ring;
+    raw.advance(set, raws);
+    // MMA blocks before this set's first block
+    ring.advance((cur.item - (int)blockIdx.x) / (int)gridDim.x * nkb + 2 * cur.kb, stages);
+    bool ok = true;
+    while (ok && cur.item < total) {
+      if (ahead.step(sets, nraw)) row = scale_row(ahead.item);
+      load_scales(row, ahead.kb, s2);
+      ok = ptx::mbar_wait(&sm.raw_full[raw.i], raw.phase, abort_flag);
+      uint4 w[4];
+      const uint8_t* src = sR + raw.i * Q4_RAW_BYTES + rr * Q4_RAW_ROW;
+      if (ok)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4*>(src + ((c ^ ((rr >> 1) & 3)) << 4));
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sm.raw_empty[raw.i]);
+      raw.advance(sets, raws);
+      const int halves = min(2, nkb - 2 * cur.kb);  // the last block may have one half
+      Ring at = ring;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h >= halves) break;
+        ok = ok && ptx::mbar_wait(&sm.empty[at.i], at.phase ^ 1, abort_flag);
+        if (ok) {
+          uint8_t* dst = sA + at.i * Q4_A_BYTES + r * ROW_BYTES;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const T s = s0[(2 * h + c) * NS / 4];
+            const uint32_t one = *reinterpret_cast<const uint16_t*>(&s);
+            const uint4 q = w[2 * h + c];
+            const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(dst + (((4 * c + k) ^ (r & 7)) << 4)) =
+                  decode_word<T>(words[k], one | (one << 16));
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sm.full[at.i]);
+        at.advance(1, stages);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        s0[j] = s1[j];
+        s1[j] = s2[j];
+      }
+      const Walk was = cur;
+      cur.step(sets, nraw);
+      ring.advance((cur.item - was.item) / (int)gridDim.x * nkb + 2 * (cur.kb - was.kb), stages);
     }
     if (!ok) {
       if (lane == 0) raise_device_error(3);
@@ -511,29 +557,27 @@ __global__ void __launch_bounds__(Q4_THREADS, 1)
   }
 }
 
-size_t int4_gemm_smem(int E) {
-  return 1024 + (size_t)Q4_SA * Q4_A_BYTES + (size_t)Q4_SX * Q4_X_BYTES + (size_t)Q4_SR * Q4_RAW_BYTES +
+size_t int4_gemm_smem(const Int4Shape& s, int E) {
+  return 1024 + (size_t)s.stages * (Q4_A_BYTES + s.nmax * ROW_BYTES) + (size_t)s.raw * Q4_RAW_BYTES +
          sizeof(Int4Smem) + 2 * (size_t)(E + 1) * sizeof(int32_t);
 }
 
 template <typename T, int GROUP, bool SWIGLU>
-int launch_int4_gemm(const CUtensorMap& tw, const CUtensorMap& tx, const Int4Params& p, int64_t items_ub,
-                     cudaStream_t st) {
-  const size_t smem = int4_gemm_smem(p.E);
+int launch_int4_gemm(const Int4Maps& maps, const Int4Params& p, int64_t items_ub, cudaStream_t st) {
+  const size_t smem = int4_gemm_smem(p.shape, p.E);
   auto kfn = int4_gemm_kernel<T, GROUP, SWIGLU>;
   MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const unsigned grid = (unsigned)std::min<int64_t>(num_sms(), items_ub);
-  MOE_CUDA_TRY(launch_kernel(kfn, dim3(grid), dim3(Q4_THREADS), smem, st, tw, tx, p));
+  MOE_CUDA_TRY(launch_kernel(kfn, dim3(grid), dim3(32 * (Q4_FIRST + 4 * p.shape.sets)), smem, st, maps, p));
   MOE_LAUNCH_CHECK("int4_gemm_kernel");
   return MOE_OK;
 }
 
 template <typename T, bool SWIGLU>
-int launch_int4_group(int group, const CUtensorMap& tw, const CUtensorMap& tx, const Int4Params& p, int64_t items_ub,
-                      cudaStream_t st) {
-  if (group == 128) return launch_int4_gemm<T, 128, SWIGLU>(tw, tx, p, items_ub, st);
-  if (group == 64) return launch_int4_gemm<T, 64, SWIGLU>(tw, tx, p, items_ub, st);
-  return launch_int4_gemm<T, 32, SWIGLU>(tw, tx, p, items_ub, st);
+int launch_int4_group(int group, const Int4Maps& maps, const Int4Params& p, int64_t items_ub, cudaStream_t st) {
+  if (group == 128) return launch_int4_gemm<T, 128, SWIGLU>(maps, p, items_ub, st);
+  if (group == 64) return launch_int4_gemm<T, 64, SWIGLU>(maps, p, items_ub, st);
+  return launch_int4_gemm<T, 32, SWIGLU>(maps, p, items_ub, st);
 }
 
 // 4-bit words of all experts: boxes of 64 bytes (128 k) by `box_rows` rows.
@@ -556,7 +600,7 @@ int make_tmap_words(CUtensorMap* m, const void* ptr, uint64_t row_bytes, uint64_
 }  // namespace
 
 bool int4_gemm_fits(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
-  const int64_t items = (ceil_div(rows, Q4_ROWS) + E) * ceil_div(n_out, Q4_FEAT / 2);
+  const int64_t items = (ceil_div(rows, kInt4Narrow.nmax) + E) * ceil_div(n_out, Q4_FEAT / 2);
   return rows < (int64_t(1) << 31) - 256 && (int64_t)E * w_rows < (int64_t(1) << 31) - 256 &&
          items < (int64_t(1) << 31) - 65536;
 }
@@ -564,10 +608,12 @@ bool int4_gemm_fits(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
 int int4_gemm(const void* x, int dtype, int64_t rows, int64_t k, const uint8_t* w, const void* scale, int group, int E,
               int64_t n_out, bool swiglu, const void* counts, int counts_is64, void* out, bool out_f32,
               cudaStream_t st) {
-  CUtensorMap tw, tx;
   const int64_t w_rows = swiglu ? 2 * n_out : n_out;
-  MOE_TRY(make_tmap_words(&tw, w, (uint64_t)k / 2, (uint64_t)E * w_rows, swiglu ? Q4_FEAT / 2 : Q4_FEAT));
-  MOE_TRY(make_tmap(&tx, x, dtype, (uint64_t)k, (uint64_t)rows, Q4_BOX));
+  const int64_t hit = std::min<int64_t>(E, rows);
+  Int4Maps maps;
+  MOE_TRY(make_tmap_words(&maps.w, w, (uint64_t)k / 2, (uint64_t)E * w_rows, swiglu ? Q4_FEAT / 2 : Q4_FEAT));
+  for (int b = 0; b < Q4_BOXES; ++b)
+    MOE_TRY(make_tmap(&maps.x[b], x, dtype, (uint64_t)k, (uint64_t)rows, 16u << b));
   Int4Params p{};
   p.E = E;
   p.K = (int)k;
@@ -581,12 +627,14 @@ int int4_gemm(const void* x, int dtype, int64_t rows, int64_t k, const uint8_t* 
   p.out = out;
   p.out_f32 = out_f32;
   p.idesc_m = make_idesc(dtype, Q4_FEAT) & ~(0x3Fu << 17);
-  const int64_t items_ub = (ceil_div(rows, Q4_ROWS) + std::min<int64_t>(E, rows)) * p.nf;
+  p.shape = rows <= kInt4NarrowRows * hit ? kInt4Narrow : kInt4Wide;
+  if (int4_gemm_smem(p.shape, E) > kMaxSmem) p.shape = kInt4WideManyExperts;
+  const int64_t items_ub = (ceil_div(rows, p.shape.nmax) + hit) * p.nf;
   if (dtype == MOE_BF16)
-    return swiglu ? launch_int4_group<__nv_bfloat16, true>(group, tw, tx, p, items_ub, st)
-                  : launch_int4_group<__nv_bfloat16, false>(group, tw, tx, p, items_ub, st);
-  return swiglu ? launch_int4_group<__half, true>(group, tw, tx, p, items_ub, st)
-                : launch_int4_group<__half, false>(group, tw, tx, p, items_ub, st);
+    return swiglu ? launch_int4_group<__nv_bfloat16, true>(group, maps, p, items_ub, st)
+                  : launch_int4_group<__nv_bfloat16, false>(group, maps, p, items_ub, st);
+  return swiglu ? launch_int4_group<__half, true>(group, maps, p, items_ub, st)
+                : launch_int4_group<__half, false>(group, maps, p, items_ub, st);
 }
 
 }  // namespace moe
