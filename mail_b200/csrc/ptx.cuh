@@ -57,6 +57,37 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t addr, uint32_t parity) {
   return ok != 0;
 }
 
+// One look, without waiting: started early, its answer is there when needed.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait that sleeps for NS nanoseconds between looks, for roles that wait
+// long beside warps that need the issue slots.
+template <int NS>
+__device__ __forceinline__ bool mbar_wait_sleepy(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                                 uint64_t timeout_ns = MOE_WAIT_TIMEOUT_NS) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      __nanosleep(NS);
+      if (mbar_test_wait(bar, parity)) return true;
+    }
+    if (*abort) return false;
+    if (globaltimer() - t0 > timeout_ns) return false;
+  }
+}
+
 // Wait until the phase with the given parity has completed. Returns false
 // after timeout_ns of global time or when *abort is raised by another role of
 // the same CTA.
