@@ -17,54 +17,115 @@ using u4::Act;
 //   s = T(absmax / 7)  (fp32 quotient, then the scales' type)
 //   q = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0
 // GROUP / 8 lanes share a group; a lane loads eight weights and stores their
-// four bytes. The rounding is that of the exact quotient (half to even): the
-// sign of w - (f + 1/2) s, one fma and so exact, decides between f and f + 1
-// where f is the floor of the rounded quotient.
+// four bytes. The rounding is that of the exact quotient, half to even. For
+// 16-bit weights the correctly rounded fp32 quotient (a reciprocal for the
+// group, then one correction by the exact remainder) is enough: a quotient of
+// two such numbers that is not on a border is further from it than fp32's
+// rounding. For fp32 weights the remainder w - i s (one fma; exact) tells
+// whether a neighbour of i is nearer or, on the border, even.
 // A group with a NaN or an infinity, or whose scale is too large for its type,
 // gets a NaN scale and q = 8, so what it stands for shows as NaN.
-__device__ __forceinline__ int nearest_step(float w, float s) {
-  const float f = floorf(__fdiv_rn(w, s));
-  const float side = fmaf(-(f + 0.5f), s, w);
-  const int i = (int)f;
-  const int up = side > 0.f || (side == 0.f && (i & 1)) ? 1 : 0;
-  return max(-8, min(7, i + up));
-}
+//
+// Both directions stream. A division for each weight bound the quantiser by
+// its instructions, about 30 a weight; now it has about 8.
+
+// Eight weights as loaded, their largest magnitude (infinity or NaN if one is),
+// and as fp32. The bits of magnitudes are in the order of the numbers, with
+// infinity and NaN on top.
+template <typename T>
+struct Eight {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float amax() const {
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    const uint32_t m = __vmaxu2(__vmaxu2(raw.x & kAbs, raw.y & kAbs), __vmaxu2(raw.z & kAbs, raw.w & kAbs));
+    const uint16_t top = (uint16_t)max(m & 0xffffu, m >> 16);
+    return Act<T>::to_float(*reinterpret_cast<const T*>(&top));
+  }
+  __device__ __forceinline__ void floats(float (&v)[8]) const { rows::load8(reinterpret_cast<const T*>(&raw), v); }
+};
+template <>
+struct Eight<float> {
+  float f[8];
+  __device__ __forceinline__ void load(const float* p) { rows::load8(p, f); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  __device__ __forceinline__ float amax() const {
+    int bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_int(f[j]) & 0x7fffffff);
+    return __int_as_float(bits);
+  }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = f[j];
+  }
+};
 
 template <typename Tw, typename Ts, int GROUP>
 __global__ void __launch_bounds__(256) quant_groups_kernel(const Tw* __restrict__ src, int64_t n8,
                                                            uint32_t* __restrict__ dst, Ts* __restrict__ scale) {
   pdl_begin();
   constexpr int kLanes = GROUP / 8;
+  constexpr int kVec = sizeof(Tw) == 2 ? 4 : 2;            // vectors of eight in flight
+  constexpr float kRound = 12582912.f;                     // 1.5 * 2^23: adding it rounds to a whole number
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;  // a multiple of kLanes: a group's lanes stay together
   const int64_t last = (n8 + 31) / 32 * 32;                // whole warps take part in the shuffles
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < last; i += stride) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (i < n8) rows::load8(src + i * 8, v);
-    float amax = 0.f;
-    bool bad = false;
+  for (int64_t base = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; base < last; base += kVec * stride) {
+    Eight<Tw> in[kVec];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      amax = fmaxf(amax, fabsf(v[j]));
-      bad |= !isfinite(v[j]);
+    for (int u = 0; u < kVec; ++u) {
+      const int64_t i = base + u * stride;
+      if (i < n8) in[u].load(src + i * 8);
+      else in[u].zero();
     }
-    if (bad) amax = INFINITY;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    Ts st = Act<Ts>::from_float(__fdiv_rn(amax, 7.0f));
-    float s = Act<Ts>::to_float(st);
-    if (!isfinite(s)) {
-      st = Act<Ts>::from_float(NAN);
-      s = 0.f;
-    }
-    uint32_t word = 0x88888888u;
-    if (s > 0.f) {
-      word = 0;
+    for (int u = 0; u < kVec; ++u) {
+      const int64_t i = base + u * stride;
+      if (i >= last) break;  // the same for the whole warp
+      int bits = __float_as_int(in[u].amax());
 #pragma unroll
-      for (int j = 0; j < 8; ++j) word |= (uint32_t)(nearest_step(v[j], s) + 8) << (4 * j);
-    }
-    if (i < n8) {
-      dst[i] = word;
-      if (i % kLanes == 0) scale[i / kLanes] = st;
+      for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+      Ts st = Act<Ts>::from_float(__fdiv_rn(__int_as_float(bits), 7.0f));
+      float s = Act<Ts>::to_float(st);
+      uint32_t word = 0x88888888u;
+      if (!isfinite(s)) {
+        st = Act<Ts>::from_float(NAN);
+      } else if (s > 0.f) {
+        float v[8];
+        in[u].floats(v);
+        if (s < 6.2e-5f) {
+          // a scale that may be subnormal: it can be well below absmax / 7, so
+          // the steps are clamped, and its reciprocal may overflow
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -8.f * s), 7.f * s) * 0x1p64f;
+          s *= 0x1p64f;
+        }
+        const float inv = __frcp_rn(s);
+        word = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float t;  // kRound + the step
+          if constexpr (sizeof(Tw) == 2) {
+            const float quot = v[j] * inv;
+            t = fmaf(fmaf(-quot, s, v[j]), inv, quot) + kRound;
+          } else {
+            t = fmaf(v[j], inv, kRound);
+            const float rest = fmaf(kRound - t, s, v[j]);
+            const float past = fmaf(2.f, fabsf(rest), -s);  // > 0: beyond half a step, 0: on the border
+            if (past > 0.f || (past == 0.f && (__float_as_int(t) & 1))) t += rest > 0.f ? 1.f : -1.f;
+          }
+          word += (uint32_t)(__float_as_int(t) - __float_as_int(kRound)) << (4 * j);
+        }
+        word += 0x88888888u;  // eight carries at most: a step is in -8 .. 7
+      }
+      if (i < n8) {
+        dst[i] = word;
+        if (i % kLanes == 0) scale[i / kLanes] = st;
+      }
     }
   }
 }
@@ -74,13 +135,27 @@ __global__ void __launch_bounds__(256) dequant_groups_kernel(const uint32_t* __r
                                                              const Ts* __restrict__ scale, int64_t n8,
                                                              To* __restrict__ dst) {
   pdl_begin();
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t)gridDim.x * blockDim.x) {
-    const uint32_t w = src[i];
-    const float s = Act<Ts>::to_float(scale[i / (GROUP / 8)]);
-    float v[8];
+  constexpr int kVec = 4;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t base = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; base < n8; base += kVec * stride) {
+    uint32_t w[kVec];
+    float s[kVec];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * s;
-    rows::store8(dst + i * 8, v);
+    for (int u = 0; u < kVec; ++u) {
+      const int64_t i = base + u * stride;
+      w[u] = i < n8 ? src[i] : 0u;
+      s[u] = i < n8 ? Act<Ts>::to_float(scale[i / (GROUP / 8)]) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kVec; ++u) {
+      const int64_t i = base + u * stride;
+      if (i >= n8) break;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)  // 2^23 + q, exactly
+        v[j] = (__int_as_float((int)((w[u] >> (4 * j)) & 15u) | 0x4b000000) - 8388616.f) * s[u];
+      rows::store8(dst + i * 8, v);
+    }
   }
 }
 
