@@ -612,8 +612,6 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
         const uint32_t s1 = ld_shared2(scale0 + slot * kScaleBytes + (NS == 2 ? 2 * half : 0));
         s01 = __byte_perm(s1, s1, 0x1010);
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sm.raw_empty[slot]);
       ok = int4_wait<20>(freed, &sm.empty[stage], phase ^ 1, abort_flag);
       if (!ok) break;
       // The loop stays rolled: the roles of this kernel run side by side from
@@ -633,7 +631,12 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sm.full[stage]);
+      if (lane == 0) {
+        ptx::mbar_arrive(&sm.full[stage]);
+        // only now: an arrive overtakes shared loads whose values nothing has
+        // waited for, and the slot's next words came in under them
+        ptx::mbar_arrive(&sm.raw_empty[slot]);
+      }
       if (stage >= kSets) {
         stage = set;
         phase ^= 1;

@@ -201,12 +201,110 @@ struct MvParams {
   int x_div;
 };
 
+// Two weight rows' words and scales of a block of 128 k, as a lane holds them.
+template <typename T, int GROUP>
+struct Block4 {
+  static constexpr int kWords = GROUP / 32;  // 32-bit words a lane holds of a row and group
+  static constexpr int kPer = 128 / GROUP;   // groups in the block
+  uint32_t q[2][4];
+  T s[2][kPer];
+};
+
+// Streamed once: not kept in L1, and the rest of a row's 256 bytes fetched into
+// L2 with it. (Narrower loads share sectors with their neighbours in L1.)
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&v)[4]) {
+  asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "l"(p));
+}
+
+// w0, w1: this lane's first words of its two rows; sc0, sc1 the rows' scales;
+// groups past the end read as q = 8 and scale 0.
+template <typename T, int GROUP>
+__device__ __forceinline__ void load_block(Block4<T, GROUP>& k, const uint8_t* w0, const uint8_t* w1, const T* sc0,
+                                           const T* sc1, int b, int groups) {
+  using B = Block4<T, GROUP>;
+#pragma unroll
+  for (int j = 0; j < B::kPer; ++j) {
+    const int g = b * B::kPer + j;
+    if (g < groups) {
+      k.s[0][j] = sc0[g];
+      k.s[1][j] = sc1[g];
+      const int64_t at = (int64_t)g * (GROUP / 2);
+      if constexpr (GROUP == 128) {
+        load_words(w0 + at, k.q[0]);
+        load_words(w1 + at, k.q[1]);
+      } else if constexpr (GROUP == 64) {
+        *reinterpret_cast<uint2*>(&k.q[0][2 * j]) = __ldg(reinterpret_cast<const uint2*>(w0 + at));
+        *reinterpret_cast<uint2*>(&k.q[1][2 * j]) = __ldg(reinterpret_cast<const uint2*>(w1 + at));
+      } else {
+        k.q[0][j] = __ldg(reinterpret_cast<const uint32_t*>(w0 + at));
+        k.q[1][j] = __ldg(reinterpret_cast<const uint32_t*>(w1 + at));
+      }
+    } else {
+      k.s[0][j] = k.s[1][j] = Act<T>::from_float(0.f);
+#pragma unroll
+      for (int i = 0; i < B::kWords; ++i) k.q[0][j * B::kWords + i] = k.q[1][j * B::kWords + i] = 0x88888888u;
+    }
+  }
+}
+
+// The activations of eight rows for the block: this lane's row, its words' k.
+template <typename T, int GROUP>
+__device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int groups) {
+  using B = Block4<T, GROUP>;
+#pragma unroll
+  for (int j = 0; j < B::kPer; ++j)
+#pragma unroll
+    for (int i = 0; i < B::kWords; ++i) {
+      const int g = b * B::kPer + j;
+      v[j * B::kWords + i] = x != nullptr && g < groups
+                                 ? *reinterpret_cast<const uint4*>(x + (int64_t)g * GROUP + i * 8)
+                                 : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// acc += the block's products: sixteen weight rows by 8 NT tokens.
+template <typename T, int GROUP, int NT>
+__device__ __forceinline__ void multiply_block(float (&acc)[NT][4], const Block4<T, GROUP>& k,
+                                               const uint4 (&x)[NT][4]) {
+  using B = Block4<T, GROUP>;
+#pragma unroll
+  for (int j = 0; j < B::kPer; ++j) {
+    float part[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < B::kWords; ++i) {
+      uint32_t a0[4], a1[4];
+      Act<T>::decode(k.q[0][j * B::kWords + i], a0);
+      Act<T>::decode(k.q[1][j * B::kWords + i], a1);
+      const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t bx[4];
+        u4::pair_up(x[n][j * B::kWords + i], bx);
+        Act<T>::mma(part[n], lo, bx[0], bx[1]);
+        Act<T>::mma(part[n], hi, bx[2], bx[3]);
+      }
+    }
+    const float s0 = Act<T>::to_float(k.s[0][j]), s1 = Act<T>::to_float(k.s[1][j]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
+      acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
+      acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
+      acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+    }
+  }
+}
+
 template <typename T, int GROUP, int NT, bool SWIGLU>
 __global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p) {
   pdl_begin();
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
-  constexpr int kPer = 128 / GROUP;       // groups of a block of 128 k
   constexpr int kTokens = 8 * NT;
+  constexpr int kDeep = NT == 1 ? 2 : 1;  // blocks in flight for a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   __shared__ int s_list[kMaxSlots];
@@ -301,7 +399,7 @@ __global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p)
     r0 = min(strip * 16 + g, p.n_out - 1);
     r1 = min(strip * 16 + g + 8, p.n_out - 1);
   }
-  const int64_t groups = p.K / GROUP;
+  const int groups = (int)(p.K / GROUP);
   const int64_t row0 = (int64_t)e * p.w_rows + r0, row1 = (int64_t)e * p.w_rows + r1;
   const uint8_t* w0 = p.w + row0 * (p.K / 2) + t * 4 * kWords;
   const uint8_t* w1 = p.w + row1 * (p.K / 2) + t * 4 * kWords;
@@ -330,61 +428,18 @@ __global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p)
       xp[n] = xr >= 0 ? x + xr * p.K + t * 8 * kWords : nullptr;
     }
     if (strip < strips) {
-#pragma unroll 2
-      for (int b = b0; b < b1; ++b) {
-        uint32_t q0[kPer][kWords], q1[kPer][kWords];
-        float s0[kPer], s1[kPer];
+      for (int b = b0; b < b1; b += kDeep) {
+        Block4<T, GROUP> k[kDeep];
+        uint4 xv[kDeep][NT][4];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int64_t grp = (int64_t)b * kPer + j;
-          const bool in = grp < groups;
-          s0[j] = in ? Act<T>::to_float(sc0[grp]) : 0.f;
-          s1[j] = in ? Act<T>::to_float(sc1[grp]) : 0.f;
-          const int64_t at = grp * (GROUP / 2);
+        for (int u = 0; u < kDeep; ++u) {
+          const int limit = b + u < b1 ? groups : 0;  // blocks past the share read as nothing
+          load_block<T, GROUP>(k[u], w0, w1, sc0, sc1, b + u, limit);
 #pragma unroll
-          for (int i = 0; i < kWords; ++i) q0[j][i] = q1[j][i] = 0x88888888u;
-          if (in) {
-            if constexpr (kWords == 4) {
-              *reinterpret_cast<uint4*>(q0[j]) = __ldg(reinterpret_cast<const uint4*>(w0 + at));
-              *reinterpret_cast<uint4*>(q1[j]) = __ldg(reinterpret_cast<const uint4*>(w1 + at));
-            } else if constexpr (kWords == 2) {
-              *reinterpret_cast<uint2*>(q0[j]) = __ldg(reinterpret_cast<const uint2*>(w0 + at));
-              *reinterpret_cast<uint2*>(q1[j]) = __ldg(reinterpret_cast<const uint2*>(w1 + at));
-            } else {
-              q0[j][0] = __ldg(reinterpret_cast<const uint32_t*>(w0 + at));
-              q1[j][0] = __ldg(reinterpret_cast<const uint32_t*>(w1 + at));
-            }
-          }
+          for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[u][n], xp[n], b + u, limit);
         }
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int64_t grp = (int64_t)b * kPer + j;
-          const bool in = grp < groups;
-          float part[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            uint32_t a0[4], a1[4];
-            Act<T>::decode(q0[j][i], a0);
-            Act<T>::decode(q1[j][i], a1);
-            const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              uint32_t bx[4] = {0u, 0u, 0u, 0u};
-              if (in && xp[n]) u4::pair_up(*reinterpret_cast<const uint4*>(xp[n] + grp * GROUP + i * 8), bx);
-              Act<T>::mma(part[n], lo, bx[0], bx[1]);
-              Act<T>::mma(part[n], hi, bx[2], bx[3]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[n][0] = fmaf(s0[j], part[n][0], acc[n][0]);
-            acc[n][1] = fmaf(s0[j], part[n][1], acc[n][1]);
-            acc[n][2] = fmaf(s1[j], part[n][2], acc[n][2]);
-            acc[n][3] = fmaf(s1[j], part[n][3], acc[n][3]);
-          }
-        }
+        for (int u = 0; u < kDeep; ++u) multiply_block<T, GROUP, NT>(acc, k[u], xv[u]);
       }
     }
 #pragma unroll

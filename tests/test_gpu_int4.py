@@ -250,6 +250,21 @@ def test_grouped_matmul_weights_past_32_bit_offsets(kernel):
     assert torch.equal(mb.grouped_matmul_int4(x, packed.transpose(1, 2), s, sizes), ref.to(BF))
 
 
+@pytest.mark.parametrize("dtype,E,K,N,group,sizes", [
+    (BF, 2, 4096, 36864, 128, [0, 2]), (BF, 2, 4096, 36864, 32, [3, 0]), (HF, 16, 2048, 6144 + 130, 64, [20] * 16),
+    (BF, 3, 4096, 16384, 128, [700, 1, 600]), (HF, 3, 4096, 16384, 32, [700, 1, 600]),
+    (BF, 3, 4096, 16384, 64, [300, 256, 600])])
+def test_grouped_matmul_long_pipelines(dtype, E, K, N, group, sizes, kernel):
+    """Many tiles of many blocks for each CTA, again and again: a stage that is
+    refilled while it is read shows here."""
+    w, s, wide = weights(E, N, K, group, dtype, 7, exact=True)
+    x = small_ints((sum(sizes), K), dtype, 8)
+    ref = grouped_ref(x, wide, sizes)[0].to(dtype)
+    gs = torch.tensor(sizes, device=DEV)
+    for _ in range(10 if kernel == "tiles" else 2):
+        assert torch.equal(mb.grouped_matmul_int4(x, w, s, gs), ref)
+
+
 def test_grouped_matmul_strided_inputs_and_other_layouts(kernel):
     w, s, wide = weights(3, 48, 256, 64, BF, 5, exact=True)
     sizes = torch.tensor([2, 0, 3], device=DEV)
