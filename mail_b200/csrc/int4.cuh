@@ -21,6 +21,13 @@ __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
+// (v & mask) | bits in one instruction; written in C the two constants cost two.
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+  return r;
+}
+
 // The 16-bit activation types.
 template <typename T>
 struct Act;
@@ -32,15 +39,22 @@ struct Act<__nv_bfloat16> {
   static __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4]) {
     const __nv_bfloat162 off = as_bf162(0x43084308u);  // 136
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = as_u32(__hsub2(as_bf162(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u), off));
+    for (int i = 0; i < 4; ++i) p[i] = as_u32(__hsub2(as_bf162(and_or(w >> (4 * i), 0x000f000fu, 0x43004300u)), off));
   }
   static __device__ __forceinline__ uint32_t scale2(uint32_t p, uint32_t s2) {
     return as_u32(__hmul2(as_bf162(p), as_bf162(s2)));
   }
   static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+  // d = a b, or d += a b
+  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -56,18 +70,25 @@ struct Act<__half> {
     const __half2 off = as_half2(0x64086408u);   // 1032
     const __half2 sixteenth = as_half2(0x2c002c00u), off16 = as_half2(0xd480d480u);  // 1 / 16, -72
     const uint32_t v = w >> 8;
-    p[0] = as_u32(__hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), off));
-    p[1] = as_u32(__hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
-    p[2] = as_u32(__hsub2(as_half2((v & 0x000f000fu) | 0x64006400u), off));
-    p[3] = as_u32(__hfma2(as_half2((v & 0x00f000f0u) | 0x64006400u), sixteenth, off16));
+    p[0] = as_u32(__hsub2(as_half2(and_or(w, 0x000f000fu, 0x64006400u)), off));
+    p[1] = as_u32(__hfma2(as_half2(and_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
+    p[2] = as_u32(__hsub2(as_half2(and_or(v, 0x000f000fu, 0x64006400u)), off));
+    p[3] = as_u32(__hfma2(as_half2(and_or(v, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
   }
   static __device__ __forceinline__ uint32_t scale2(uint32_t p, uint32_t s2) {
     return as_u32(__hmul2(as_half2(p), as_half2(s2)));
   }
   static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+  // d = a b, or d += a b
+  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));

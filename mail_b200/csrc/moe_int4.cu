@@ -6,6 +6,7 @@
 #include "common.cuh"
 #include "int4.cuh"
 #include "rows.cuh"
+#include "scan.cuh"
 
 namespace moe {
 namespace {
@@ -164,12 +165,14 @@ __global__ void __launch_bounds__(256) dequant_groups_kernel(const uint32_t* __r
 //   out[r, n] = sum_k x[r, k] W[e(r), n, k]
 // SWIGLU: W holds I gate rows and I up rows and out[r, n] = silu(g) u.
 //
-// One CTA takes a strip of weight rows of one expert and all of the expert's
-// rows, eight at a time per mma (m16n8k16: sixteen weight rows by eight
-// tokens). Its eight warps are WM strips of sixteen weight rows by WK shares
-// of K; the shares are added through shared memory in the order of the warps,
-// so results do not depend on timing. With SWIGLU a strip's sixteen rows are
-// eight gate rows and the eight up rows that go with them.
+// A strip of sixteen weight rows of an expert, eight of its rows at a time, is
+// an mma tile (m16n8k16). The grid is persistent: each CTA first lists the
+// experts that have rows, then its groups of `wk` warps take strips in turn,
+// each warp of a group a share of K; the shares are added through shared memory
+// in the order of the warps, so results do not depend on timing. With SWIGLU a
+// strip's sixteen rows are eight gate rows and the eight up rows that go with
+// them. (A CTA for each strip and possible expert, most of which leave at once,
+// took 93 us for two rows of 4096 over eight experts of 28672 rows.)
 //
 // A lane (row g = lane / 4, t = lane % 4) loads GROUP / 4 consecutive k of its
 // two weight rows at a time, so that the four lanes of a row cover exactly one
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(256) dequant_groups_kernel(const uint32_t* __r
 // which rounds no weight.
 constexpr int kMvThreads = 256;
 constexpr int kMvWarps = kMvThreads / 32;
+constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 1024;  // routed slots of the form that reads top-k ids
 
 struct MvParams {
@@ -188,7 +192,7 @@ struct MvParams {
   int64_t K;
   int n_out, w_rows;     // output features; weight rows of an expert (2 n_out with SWIGLU)
   int E;
-  int wk;                // shares of K (1, 2, 4 or 8)
+  int wk;                // warps that share a strip along K (1, 2, 4 or 8)
   int out_f32;           // out is fp32, else the activations' type
   // rows: either the top-k ids of `slots` slots (row r of x is slot / x_div, row
   // of out is the slot), or counts of consecutive rows
@@ -273,8 +277,6 @@ __device__ __forceinline__ void multiply_block(float (&acc)[NT][4], const Block4
   for (int j = 0; j < B::kPer; ++j) {
     float part[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
-#pragma unroll
     for (int i = 0; i < B::kWords; ++i) {
       uint32_t a0[4], a1[4];
       Act<T>::decode(k.q[0][j * B::kWords + i], a0);
@@ -284,7 +286,8 @@ __device__ __forceinline__ void multiply_block(float (&acc)[NT][4], const Block4
       for (int n = 0; n < NT; ++n) {
         uint32_t bx[4];
         u4::pair_up(x[n][j * B::kWords + i], bx);
-        Act<T>::mma(part[n], lo, bx[0], bx[1]);
+        if (i == 0) Act<T>::mma_first(part[n], lo, bx[0], bx[1]);
+        else Act<T>::mma(part[n], lo, bx[0], bx[1]);
         Act<T>::mma(part[n], hi, bx[2], bx[3]);
       }
     }
@@ -299,141 +302,151 @@ __device__ __forceinline__ void multiply_block(float (&acc)[NT][4], const Block4
   }
 }
 
+// The experts that have rows, in order: expert, first place in the list of
+// rows, number of rows. Rows in counts form are the places themselves; in ids
+// form s.list holds the slots expert by expert (in no particular order).
+struct RowLists {
+  int expert[kMaxExperts], first[kMaxExperts], rows[kMaxExperts];
+  int list[kMaxSlots];
+  int total;   // rows in all
+  int active;  // experts listed
+};
+
+__device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
+  __shared__ int64_t warp_sums[32];
+  const int tid = threadIdx.x;
+  const int per = (p.E + kMvThreads - 1) / kMvThreads;
+  const int lo = min(p.E, tid * per), hi = min(p.E, lo + per);
+  if (p.ids) {
+    for (int e = tid; e < p.E; e += kMvThreads) s.rows[e] = 0;
+    __syncthreads();
+    for (int i = tid; i < p.slots; i += kMvThreads) {
+      const int e = p.ids[i];
+      if (e >= 0 && e < p.E) atomicAdd(&s.rows[e], 1);
+    }
+    __syncthreads();
+  }
+  int cnt[kMaxExperts / kMvThreads];
+  int64_t mine = 0;  // rows << 11 | experts that have some
+#pragma unroll
+  for (int i = 0; i < kMaxExperts / kMvThreads; ++i) {
+    cnt[i] = 0;
+    if (lo + i < hi) {
+      if (p.ids) {
+        cnt[i] = s.rows[lo + i];
+      } else {
+        const int64_t c = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[lo + i]
+                                        : (int64_t) static_cast<const int32_t*>(p.counts)[lo + i];
+        cnt[i] = (int)max((int64_t)0, min(c, p.total_rows));
+      }
+      mine += ((int64_t)cnt[i] << 11) + (cnt[i] > 0);
+    }
+  }
+  const int64_t incl = block_inclusive_scan<int64_t>(mine, warp_sums);  // ends with a barrier: rows[] may be reused
+  const int64_t limit = p.ids ? (int64_t)p.slots : p.total_rows;
+  int64_t run = (incl - mine) >> 11;
+  int a = (int)((incl - mine) & 2047);
+#pragma unroll
+  for (int i = 0; i < kMaxExperts / kMvThreads; ++i) {
+    if (cnt[i] > 0) {  // counts past the last row are cut off
+      s.expert[a] = lo + i;
+      s.first[a] = (int)min(run, limit);
+      s.rows[a] = (int)min((int64_t)cnt[i], max((int64_t)0, limit - run));
+      ++a;
+      run += cnt[i];
+    }
+  }
+  if (tid == kMvThreads - 1) {
+    s.total = (int)min(incl >> 11, limit);
+    s.active = (int)(incl & 2047);
+  }
+  __syncthreads();
+  if (p.ids) {
+    // a slot's place: its expert's first, then one after the other
+    for (int i = tid; i < p.slots; i += kMvThreads) {
+      const int e = p.ids[i];
+      if (e < 0 || e >= p.E) continue;
+      int l = 0, h = s.active - 1;
+      while (l < h) {
+        const int m = (l + h) >> 1;
+        if (s.expert[m] < e) l = m + 1;
+        else h = m;
+      }
+      s.list[atomicAdd(&s.first[l], 1)] = i;
+    }
+    __syncthreads();
+    for (int i = tid; i < s.active; i += kMvThreads) s.first[i] -= s.rows[i];
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ void group_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 template <typename T, int GROUP, int NT, bool SWIGLU>
-__global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p) {
+__global__ void __launch_bounds__(kMvThreads, NT == 1 ? 3 : 2) int4_rows_kernel(const MvParams p) {
   pdl_begin();
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
   constexpr int kTokens = 8 * NT;
+  constexpr int kFeat = SWIGLU ? 8 : 16;  // output features of a strip
   constexpr int kDeep = NT == 1 ? 2 : 1;  // blocks in flight for a warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  __shared__ int s_list[kMaxSlots];
-  __shared__ int s_part[kMaxSlots / 32];
-  __shared__ int64_t s_sum[kMvWarps];
-  __shared__ int64_t s_x[kTokens], s_o[kTokens];
+  __shared__ RowLists s;
   __shared__ float s_red[kMvWarps][16][kTokens + 1];
+  list_rows(s, p);
 
-  const int wm = kMvWarps / p.wk;
-  const int strips = (p.n_out + (SWIGLU ? 7 : 15)) / (SWIGLU ? 8 : 16);
-  int e;
-  int64_t off = 0, cnt = 0;
-  if (p.ids) {
-    // this CTA stands for the slot blockIdx.y; the first slot of an expert
-    // works for all of them
-    const int me = blockIdx.y;
-    e = p.ids[me];
-    if (e < 0 || e >= p.E) return;
-    const int passes = (p.slots + kMvThreads - 1) / kMvThreads;
-    bool mine[kMaxSlots / kMvThreads];
-    int before[kMaxSlots / kMvThreads];
-    bool earlier = false;
-#pragma unroll
-    for (int i = 0; i < kMaxSlots / kMvThreads; ++i) {
-      mine[i] = false;
-      before[i] = 0;
-      if (i < passes) {
-        const int s = i * kMvThreads + threadIdx.x;
-        mine[i] = s < p.slots && p.ids[s] == e;
-        earlier |= mine[i] && s < me;
-        const unsigned b = __ballot_sync(0xffffffffu, mine[i]);
-        before[i] = __popc(b & ((1u << lane) - 1));
-        if (lane == 0) s_part[i * kMvWarps + warp] = __popc(b);
-      }
-    }
-    if (__syncthreads_or(earlier)) return;
-    int run = 0;
-#pragma unroll
-    for (int i = 0; i < kMaxSlots / kMvThreads; ++i) {
-      if (i < passes) {
-        for (int w = 0; w < kMvWarps; ++w) {
-          if (w == warp && mine[i]) s_list[run + before[i]] = i * kMvThreads + threadIdx.x;
-          run += s_part[i * kMvWarps + w];
-        }
-      }
-    }
-    cnt = run;
-    __syncthreads();
-  } else {
-    e = blockIdx.y;  // e == E: the rows that no expert has
-    int64_t sum = 0;
-    for (int i = threadIdx.x; i < min(e, p.E); i += kMvThreads) {
-      const int64_t c = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[i]
-                                      : (int64_t) static_cast<const int32_t*>(p.counts)[i];
-      sum += max(c, (int64_t)0);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    for (int w = 0; w < kMvWarps; ++w) off += s_sum[w];
-    off = min(off, p.total_rows);
-    if (e == p.E) {
-      const int es = p.out_f32 ? 4 : 2;
-      const int64_t n0 = (int64_t)blockIdx.x * wm * (SWIGLU ? 8 : 16);
-      const int64_t n1 = min((int64_t)p.n_out, n0 + wm * (SWIGLU ? 8 : 16));
-      for (int64_t r = off; r < p.total_rows; ++r)
-        for (int64_t n = n0 + threadIdx.x; n < n1; n += kMvThreads) {
-          if (es == 4) static_cast<float*>(p.out)[r * p.n_out + n] = 0.f;
-          else static_cast<uint16_t*>(p.out)[r * p.n_out + n] = 0;
-        }
-      return;
-    }
-    cnt = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[e]
-                        : (int64_t) static_cast<const int32_t*>(p.counts)[e];
-    cnt = max((int64_t)0, min(cnt, p.total_rows - off));
-    if (cnt == 0) return;
-  }
-
-  const int sm = warp / p.wk, share = warp % p.wk;  // strip of this warp, its share of K
-  const int strip = blockIdx.x * wm + sm;
+  const int wk = p.wk;
+  const int groups_in_cta = kMvWarps / wk, group = warp / wk, share = warp % wk;
+  const int strips = (p.n_out + kFeat - 1) / kFeat;
   const int blocks = (int)((p.K + 127) / 128);
-  const int b0 = (int)((int64_t)blocks * share / p.wk), b1 = (int)((int64_t)blocks * (share + 1) / p.wk);
-  // rows of W of this lane: row g and row g + 8 of the strip (rows past the
-  // end read the last row and are not stored)
-  int r0, r1;
-  if (SWIGLU) {
-    const int f = min(strip * 8 + g, p.n_out - 1);
-    r0 = f;
-    r1 = p.n_out + f;
-  } else {
-    r0 = min(strip * 16 + g, p.n_out - 1);
-    r1 = min(strip * 16 + g + 8, p.n_out - 1);
-  }
-  const int groups = (int)(p.K / GROUP);
-  const int64_t row0 = (int64_t)e * p.w_rows + r0, row1 = (int64_t)e * p.w_rows + r1;
-  const uint8_t* w0 = p.w + row0 * (p.K / 2) + t * 4 * kWords;
-  const uint8_t* w1 = p.w + row1 * (p.K / 2) + t * 4 * kWords;
-  const T* sc0 = static_cast<const T*>(p.scale) + row0 * groups;
-  const T* sc1 = static_cast<const T*>(p.scale) + row1 * groups;
+  const int b0 = (int)((int64_t)blocks * share / wk), b1 = (int)((int64_t)blocks * (share + 1) / wk);
+  const int kgroups = (int)(p.K / GROUP);
   const T* x = static_cast<const T*>(p.x);
+  const int64_t units = (int64_t)s.active * strips;
+  const int64_t stride = (int64_t)gridDim.x * groups_in_cta;
 
-  for (int64_t c0 = 0; c0 < cnt; c0 += kTokens) {
-    if (threadIdx.x < kTokens) {
-      const int64_t i = c0 + threadIdx.x;
-      int64_t xr = -1, orow = -1;
-      if (i < cnt) {
-        orow = p.ids ? (int64_t)s_list[i] : off + i;
-        xr = p.ids ? orow / p.x_div : (p.row_map ? (int64_t)(p.row_map[orow] / p.x_div) : orow);
-      }
-      s_x[threadIdx.x] = xr;
-      s_o[threadIdx.x] = orow;
+  // neighbouring units on different CTAs: a small launch spreads over the SMs
+  for (int64_t unit = (int64_t)group * gridDim.x + blockIdx.x; unit < units; unit += stride) {
+    const int a = (int)(unit / strips), strip = (int)(unit % strips);
+    const int e = s.expert[a], first = s.first[a], cnt = s.rows[a];
+    // rows of W of this lane: row g and row g + 8 of the strip (rows past the
+    // end read the last row and are not stored)
+    int r0, r1;
+    if (SWIGLU) {
+      r0 = min(strip * 8 + g, p.n_out - 1);
+      r1 = p.n_out + r0;
+    } else {
+      r0 = min(strip * 16 + g, p.n_out - 1);
+      r1 = min(strip * 16 + g + 8, p.n_out - 1);
     }
-    __syncthreads();
-    float acc[NT][4];
-    const T* xp[NT];
+    const int64_t row0 = (int64_t)e * p.w_rows + r0, row1 = (int64_t)e * p.w_rows + r1;
+    const uint8_t* w0 = p.w + row0 * (p.K / 2) + t * 4 * kWords;
+    const uint8_t* w1 = p.w + row1 * (p.K / 2) + t * 4 * kWords;
+    const T* sc0 = static_cast<const T*>(p.scale) + row0 * kgroups;
+    const T* sc1 = static_cast<const T*>(p.scale) + row1 * kgroups;
+
+    for (int c0 = 0; c0 < cnt; c0 += kTokens) {
+      float acc[NT][4];
+      const T* xp[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-      const int64_t xr = s_x[n * 8 + g];
-      xp[n] = xr >= 0 ? x + xr * p.K + t * 8 * kWords : nullptr;
-    }
-    if (strip < strips) {
+      for (int n = 0; n < NT; ++n) {
+        acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        const int i = c0 + n * 8 + g;
+        xp[n] = nullptr;
+        if (i < cnt) {
+          const int place = first + i;
+          const int row = p.ids ? s.list[place] / p.x_div : (p.row_map ? p.row_map[place] / p.x_div : place);
+          xp[n] = x + (int64_t)row * p.K + t * 8 * kWords;
+        }
+      }
       for (int b = b0; b < b1; b += kDeep) {
         Block4<T, GROUP> k[kDeep];
         uint4 xv[kDeep][NT][4];
 #pragma unroll
         for (int u = 0; u < kDeep; ++u) {
-          const int limit = b + u < b1 ? groups : 0;  // blocks past the share read as nothing
+          const int limit = b + u < b1 ? kgroups : 0;  // blocks past the share read as nothing
           load_block<T, GROUP>(k[u], w0, w1, sc0, sc1, b + u, limit);
 #pragma unroll
           for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[u][n], xp[n], b + u, limit);
@@ -441,33 +454,41 @@ __global__ void __launch_bounds__(kMvThreads) int4_rows_kernel(const MvParams p)
 #pragma unroll
         for (int u = 0; u < kDeep; ++u) multiply_block<T, GROUP, NT>(acc, k[u], xv[u]);
       }
-    }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      s_red[warp][g][n * 8 + 2 * t] = acc[n][0];
-      s_red[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
-      s_red[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
-      s_red[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
-    }
-    __syncthreads();
-    // strip m, feature f, token n: the shares added in order
-    constexpr int kFeat = SWIGLU ? 8 : 16;
-    for (int i = threadIdx.x; i < wm * kFeat * kTokens; i += kMvThreads) {
-      const int f = i % kFeat, m = i / kFeat % wm, n = i / (kFeat * wm);
-      const int feat = (blockIdx.x * wm + m) * kFeat + f;
-      const int64_t orow = s_o[n];
-      if (orow < 0 || feat >= p.n_out) continue;
-      float v = 0.f, u = 0.f;
-      for (int k = 0; k < p.wk; ++k) {
-        v += s_red[m * p.wk + k][f][n];
-        if (SWIGLU) u += s_red[m * p.wk + k][f + 8][n];
+      for (int n = 0; n < NT; ++n) {
+        s_red[warp][g][n * 8 + 2 * t] = acc[n][0];
+        s_red[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
+        s_red[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
+        s_red[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
       }
-      if (SWIGLU) v = u4::silu_mul(v, u);
-      const int64_t at = orow * p.n_out + feat;
-      if (p.out_f32) static_cast<float*>(p.out)[at] = v;
-      else static_cast<T*>(p.out)[at] = Act<T>::from_float(v);
+      group_barrier(1 + group, 32 * wk);
+      // feature f, token n: the shares added in order
+      const int tokens = min(kTokens, cnt - c0);
+      for (int i = share * 32 + lane; i < kFeat * tokens; i += 32 * wk) {
+        const int f = i % kFeat, n = i / kFeat;
+        const int feat = strip * kFeat + f;
+        if (feat >= p.n_out) continue;
+        float v = 0.f, u = 0.f;
+        for (int k = 0; k < wk; ++k) {
+          v += s_red[group * wk + k][f][n];
+          if (SWIGLU) u += s_red[group * wk + k][f + 8][n];
+        }
+        if (SWIGLU) v = u4::silu_mul(v, u);
+        const int place = first + c0 + n;
+        const int64_t at = (int64_t)(p.ids ? s.list[place] : place) * p.n_out + feat;
+        if (p.out_f32) static_cast<float*>(p.out)[at] = v;
+        else static_cast<T*>(p.out)[at] = Act<T>::from_float(v);
+      }
+      group_barrier(1 + group, 32 * wk);
     }
-    __syncthreads();
+  }
+  if (!p.ids) {  // rows behind the last expert's are zero
+    const int64_t n0 = (int64_t)s.total * p.n_out, n1 = p.total_rows * p.n_out;
+    for (int64_t i = n0 + (int64_t)blockIdx.x * kMvThreads + threadIdx.x; i < n1;
+         i += (int64_t)gridDim.x * kMvThreads) {
+      if (p.out_f32) static_cast<float*>(p.out)[i] = 0.f;
+      else static_cast<uint16_t*>(p.out)[i] = 0;
+    }
   }
 }
 
@@ -532,25 +553,23 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
 }
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
-int launch_rows_nt(MvParams p, cudaStream_t st) {
-  const int strips = (int)ceil_div(p.n_out, SWIGLU ? 8 : 16);
-  const int wm = kMvWarps / p.wk;
-  const dim3 grid((unsigned)ceil_div(strips, wm), (unsigned)(p.ids ? p.slots : p.E + 1));
-  MOE_CUDA_TRY(launch_kernel(int4_rows_kernel<T, GROUP, NT, SWIGLU>, grid, dim3(kMvThreads), 0, st, p));
+int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
+  // shares of K: as many as the launch has warps for, each at least two blocks
+  const int64_t blocks = ceil_div(p.K, 128);
+  const int64_t units = ceil_div(p.n_out, SWIGLU ? 8 : 16) * std::min<int64_t>(p.E, rows);
+  const int64_t warps = (int64_t)num_sms() * (NT == 1 ? 3 : 2) * kMvWarps;
+  p.wk = 1;
+  while (p.wk < kMvWarps && 2 * units * p.wk <= warps && blocks >= 4 * p.wk) p.wk *= 2;
+  const int64_t ctas = std::min<int64_t>(ceil_div(units, kMvWarps / p.wk), warps / kMvWarps);
+  MOE_CUDA_TRY(launch_kernel(int4_rows_kernel<T, GROUP, NT, SWIGLU>, dim3((unsigned)ctas), dim3(kMvThreads), 0, st, p));
   MOE_LAUNCH_CHECK("int4_rows_kernel");
   return MOE_OK;
 }
 
 template <typename T, int GROUP, bool SWIGLU>
-int launch_rows_group(MvParams p, int64_t rows, cudaStream_t st) {
-  // shares of K: as many as leave each warp two blocks of 128 k, fewer where
-  // the strips alone fill the device
-  const int64_t blocks = ceil_div(p.K, 128);
-  const int64_t units = ceil_div(p.n_out, SWIGLU ? 8 : 16) * std::min<int64_t>(p.E, rows);
-  p.wk = kMvWarps;
-  while (p.wk > 1 && (blocks < 2 * p.wk || units * p.wk > (int64_t)num_sms() * 64 * 4)) p.wk /= 2;
-  if (rows <= 8 || rows <= 2 * (int64_t)p.E) return launch_rows_nt<T, GROUP, 1, SWIGLU>(p, st);
-  return launch_rows_nt<T, GROUP, 4, SWIGLU>(p, st);
+int launch_rows_group(const MvParams& p, int64_t rows, cudaStream_t st) {
+  if (rows <= 8 || rows <= 2 * (int64_t)p.E) return launch_rows_nt<T, GROUP, 1, SWIGLU>(p, rows, st);
+  return launch_rows_nt<T, GROUP, 2, SWIGLU>(p, rows, st);
 }
 
 // Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM).
