@@ -4,12 +4,10 @@
 //
 // Byte b of a weight row holds q[2b] in its low and q[2b + 1] in its high
 // nibble; s is in the activations' 16-bit type. A 32-bit word so holds eight
-// consecutive k, k0 in its lowest nibble. Masking 0x000f000f at shifts of 0,
-// 4, 8 and 12 gives the pairs (k0, k4), (k1, k5), (k2, k6), (k3, k7), each
-// nibble in the low mantissa bits of a 16-bit half; setting the exponent of
-// 128 (bf16) or 1024 (fp16) there makes it the number 128 + q or 1024 + q,
-// exactly, and one packed subtraction leaves q - 8. The activations are paired
-// the same way, so the order of k inside a product does not matter.
+// consecutive k, k0 in its lowest nibble. Masking a nibble in both halves of
+// the word at once gives one of the pairs (k0, k4), (k1, k5), (k2, k6),
+// (k3, k7). Put into the mantissas of two 16-bit numbers under an exponent
+// that makes their step 1 it is the number M + q, exactly.
 #pragma once
 #include "common.cuh"
 
@@ -34,24 +32,31 @@ struct Act;
 
 template <>
 struct Act<__nv_bfloat16> {
-  static constexpr int kDtype = MOE_BF16;
-  // q - 8 of word w: pairs (k0, k4), (k1, k5), (k2, k6), (k3, k7)
+  // M + q of word w: pairs (k0, k4) with M = 128, from the lowest four mantissa
+  // bits as they stand; (k1, k5), (k2, k6), (k3, k7) with M = 16, shifted to
+  // the highest four. Left as it is, M costs no instruction for each weight;
+  // kOffset, -(M + 8), multiplied by the same
+  // activations, takes it out of the sums.
   static __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4]) {
-    const __nv_bfloat162 off = as_bf162(0x43084308u);  // 136
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = as_u32(__hsub2(as_bf162(and_or(w >> (4 * i), 0x000f000fu, 0x43004300u)), off));
+    p[0] = and_or(w, 0x000f000fu, 0x43004300u);
+    p[1] = and_or(w >> 1, 0x00780078u, 0x41804180u);
+    p[2] = and_or(w >> 5, 0x00780078u, 0x41804180u);
+    p[3] = and_or(w >> 9, 0x00780078u, 0x41804180u);
   }
-  static __device__ __forceinline__ uint32_t scale2(uint32_t p, uint32_t s2) {
-    return as_u32(__hmul2(as_bf162(p), as_bf162(s2)));
-  }
+  static constexpr uint32_t kOffset[4] = {0xc308c308u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};  // -136, -24, ..
   static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-  // d = a b, or d += a b
-  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  // d = a b + c, d = a b, d += a b
+  static __device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                  const float (&c)[4]) {
     asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  }
+  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_from(d, a, b0, b1, zero);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
@@ -63,29 +68,28 @@ struct Act<__nv_bfloat16> {
 
 template <>
 struct Act<__half> {
-  static constexpr int kDtype = MOE_F16;
+  // M + q: ten mantissa bits take (k1, k5) as it stands, with M = 64; the other
+  // pairs shifted to the highest four, with M = 16
   static __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4]) {
-    // ten mantissa bits also hold a nibble four bits up: 1024 + 16 q, which a
-    // packed fma turns into q - 8 (exact: 1024 / 16 + 8 = 72)
-    const __half2 off = as_half2(0x64086408u);   // 1032
-    const __half2 sixteenth = as_half2(0x2c002c00u), off16 = as_half2(0xd480d480u);  // 1 / 16, -72
-    const uint32_t v = w >> 8;
-    p[0] = as_u32(__hsub2(as_half2(and_or(w, 0x000f000fu, 0x64006400u)), off));
-    p[1] = as_u32(__hfma2(as_half2(and_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
-    p[2] = as_u32(__hsub2(as_half2(and_or(v, 0x000f000fu, 0x64006400u)), off));
-    p[3] = as_u32(__hfma2(as_half2(and_or(v, 0x00f000f0u, 0x64006400u)), sixteenth, off16));
+    p[0] = and_or(w << 6, 0x03c003c0u, 0x4c004c00u);
+    p[1] = and_or(w, 0x00f000f0u, 0x54005400u);
+    p[2] = and_or(w >> 2, 0x03c003c0u, 0x4c004c00u);
+    p[3] = and_or(w >> 6, 0x03c003c0u, 0x4c004c00u);
   }
-  static __device__ __forceinline__ uint32_t scale2(uint32_t p, uint32_t s2) {
-    return as_u32(__hmul2(as_half2(p), as_half2(s2)));
-  }
+  static constexpr uint32_t kOffset[4] = {0xce00ce00u, 0xd480d480u, 0xce00ce00u, 0xce00ce00u};  // -24, -72, ..
   static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-  // d = a b, or d += a b
-  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  // d = a b + c, d = a b, d += a b
+  static __device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                  const float (&c)[4]) {
     asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  }
+  static __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_from(d, a, b0, b1, zero);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(

@@ -165,20 +165,30 @@ __global__ void __launch_bounds__(256) dequant_groups_kernel(const uint32_t* __r
 //   out[r, n] = sum_k x[r, k] W[e(r), n, k]
 // SWIGLU: W holds I gate rows and I up rows and out[r, n] = silu(g) u.
 //
-// A strip of sixteen weight rows of an expert, eight of its rows at a time, is
-// an mma tile (m16n8k16). The grid is persistent: each CTA first lists the
-// experts that have rows, then its groups of `wk` warps take strips in turn,
-// each warp of a group a share of K; the shares are added through shared memory
-// in the order of the warps, so results do not depend on timing. With SWIGLU a
-// strip's sixteen rows are eight gate rows and the eight up rows that go with
-// them. (A CTA for each strip and possible expert, most of which leave at once,
-// took 93 us for two rows of 4096 over eight experts of 28672 rows.)
+// A warp works on strips of 32 weight rows of an expert, two mma tiles (m16n8k16:
+// sixteen weight rows by eight of the expert's rows). The grid is persistent:
+// each CTA first lists the experts that have rows, then its groups of `wk` warps
+// take strips in turn, each warp of a group a share of K; the shares are added
+// through shared memory in the order of the warps, so results do not depend on
+// timing. With SWIGLU a tile's sixteen rows are eight gate rows and the eight up
+// rows that go with them. (A CTA for each strip and possible expert, most of
+// which leave at once, took 93 us for two rows of 4096 over eight experts of
+// 28672 rows.)
 //
-// A lane (row g = lane / 4, t = lane % 4) loads GROUP / 4 consecutive k of its
-// two weight rows at a time, so that the four lanes of a row cover exactly one
-// group of scales: the products of a group are summed from the integers
-// q - 8, which 16-bit types hold exactly, and the fp32 sum is scaled once,
-// which rounds no weight.
+// A lane (row g = lane / 4, t = lane % 4) holds GROUP / 4 consecutive k of its
+// weight rows at a time, so that the four lanes of a row cover exactly one
+// group of scales: the products of a group are summed from whole numbers, which
+// 16-bit types hold exactly, and the fp32 sum is scaled once, which rounds no
+// weight. The numbers are M + q (int4.cuh); the mma tile of the offsets -(M + 8)
+// with the same activations comes first and serves both weight tiles, so no
+// weight is corrected by itself. The terms of the two cancel to at most 136 / 8
+// of their size (bf16; 72 / 8 in fp16), which costs the fp32 sums five bits of
+// the eight (fp16: eight) that they have to spare over a 24-bit significand
+// against the output's.
+//
+// What bounds it is the instruction rate: with one tile a warp and a subtraction
+// for each pair of weights a block of 16 x 128 weights took 192 instructions,
+// now 105.
 constexpr int kMvThreads = 256;
 constexpr int kMvWarps = kMvThreads / 32;
 constexpr int kMaxExperts = 1024;
@@ -192,7 +202,6 @@ struct MvParams {
   int64_t K;
   int n_out, w_rows;     // output features; weight rows of an expert (2 n_out with SWIGLU)
   int E;
-  int wk;                // warps that share a strip along K (1, 2, 4 or 8)
   int out_f32;           // out is fp32, else the activations' type
   // rows: either the top-k ids of `slots` slots (row r of x is slot / x_div, row
   // of out is the slot), or counts of consecutive rows
@@ -205,51 +214,62 @@ struct MvParams {
   int x_div;
 };
 
-// Two weight rows' words and scales of a block of 128 k, as a lane holds them.
+// A block of 128 k of a lane's four weight rows: rows g and g + 8 of two tiles.
 template <typename T, int GROUP>
 struct Block4 {
   static constexpr int kWords = GROUP / 32;  // 32-bit words a lane holds of a row and group
   static constexpr int kPer = 128 / GROUP;   // groups in the block
-  uint32_t q[2][4];
-  T s[2][kPer];
+  uint32_t q[4][4];
+  T s[4][kPer];
 };
+constexpr int kBlockBytes = 2048;  // of a warp in shared memory: four times 512
 
-// Streamed once: not kept in L1, and the rest of a row's 256 bytes fetched into
-// L2 with it. (Narrower loads share sectors with their neighbours in L1.)
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&v)[4]) {
-  asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-      : "l"(p));
+// Copies this lane's words of a block to its own 16 bytes for each row in
+// shared memory, asynchronously. Nobody else reads them, so waiting for the
+// copies is all the synchronisation there is. Groups past the end are left out:
+// any words will do, their scales and activations are zero.
+template <int GROUP>
+__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* const (&w)[4], int b, int groups) {
+  constexpr int kPer = 128 / GROUP, kBytes = 16 / kPer;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int g = b * kPer + j;
+    if (g < groups) {
+      const int at = g * (GROUP / 2);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (GROUP == 128)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst + r * 512), "l"(w[r] + at)
+                       : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], %2;" ::"r"(dst + r * 512 + j * kBytes),
+                       "l"(w[r] + at), "n"(kBytes)
+                       : "memory");
+      }
+    }
+  }
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void read_words(uint32_t src, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(src)
+               : "memory");
 }
 
-// w0, w1: this lane's first words of its two rows; sc0, sc1 the rows' scales;
-// groups past the end read as q = 8 and scale 0.
+// The scales of a block; 0 for groups past the end.
 template <typename T, int GROUP>
-__device__ __forceinline__ void load_block(Block4<T, GROUP>& k, const uint8_t* w0, const uint8_t* w1, const T* sc0,
-                                           const T* sc1, int b, int groups) {
+__device__ __forceinline__ void load_scales(Block4<T, GROUP>& k, const T* const (&sc)[4], int b, int groups) {
   using B = Block4<T, GROUP>;
 #pragma unroll
   for (int j = 0; j < B::kPer; ++j) {
     const int g = b * B::kPer + j;
-    if (g < groups) {
-      k.s[0][j] = sc0[g];
-      k.s[1][j] = sc1[g];
-      const int64_t at = (int64_t)g * (GROUP / 2);
-      if constexpr (GROUP == 128) {
-        load_words(w0 + at, k.q[0]);
-        load_words(w1 + at, k.q[1]);
-      } else if constexpr (GROUP == 64) {
-        *reinterpret_cast<uint2*>(&k.q[0][2 * j]) = __ldg(reinterpret_cast<const uint2*>(w0 + at));
-        *reinterpret_cast<uint2*>(&k.q[1][2 * j]) = __ldg(reinterpret_cast<const uint2*>(w1 + at));
-      } else {
-        k.q[0][j] = __ldg(reinterpret_cast<const uint32_t*>(w0 + at));
-        k.q[1][j] = __ldg(reinterpret_cast<const uint32_t*>(w1 + at));
-      }
-    } else {
-      k.s[0][j] = k.s[1][j] = Act<T>::from_float(0.f);
 #pragma unroll
-      for (int i = 0; i < B::kWords; ++i) k.q[0][j * B::kWords + i] = k.q[1][j * B::kWords + i] = 0x88888888u;
-    }
+    for (int r = 0; r < 4; ++r) k.s[r][j] = g < groups ? sc[r][g] : Act<T>::from_float(0.f);
   }
 }
 
@@ -268,36 +288,50 @@ __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int 
     }
 }
 
-// acc += the block's products: sixteen weight rows by 8 NT tokens.
+// acc += the block's products: two tiles of sixteen weight rows by 8 NT tokens.
 template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void multiply_block(float (&acc)[NT][4], const Block4<T, GROUP>& k,
+__device__ __forceinline__ void multiply_block(float (&acc)[2][NT][4], const Block4<T, GROUP>& k,
                                                const uint4 (&x)[NT][4]) {
   using B = Block4<T, GROUP>;
+  constexpr uint32_t off_lo[4] = {Act<T>::kOffset[0], Act<T>::kOffset[0], Act<T>::kOffset[1], Act<T>::kOffset[1]};
+  constexpr uint32_t off_hi[4] = {Act<T>::kOffset[2], Act<T>::kOffset[2], Act<T>::kOffset[3], Act<T>::kOffset[3]};
 #pragma unroll
   for (int j = 0; j < B::kPer; ++j) {
-    float part[NT][4];
+    uint32_t bx[B::kWords][NT][4];
+    float base[NT][4];
 #pragma unroll
-    for (int i = 0; i < B::kWords; ++i) {
-      uint32_t a0[4], a1[4];
-      Act<T>::decode(k.q[0][j * B::kWords + i], a0);
-      Act<T>::decode(k.q[1][j * B::kWords + i], a1);
-      const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
+    for (int i = 0; i < B::kWords; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        uint32_t bx[4];
-        u4::pair_up(x[n][j * B::kWords + i], bx);
-        if (i == 0) Act<T>::mma_first(part[n], lo, bx[0], bx[1]);
-        else Act<T>::mma(part[n], lo, bx[0], bx[1]);
-        Act<T>::mma(part[n], hi, bx[2], bx[3]);
+        u4::pair_up(x[n][j * B::kWords + i], bx[i][n]);
+        if (i == 0) Act<T>::mma_first(base[n], off_lo, bx[i][n][0], bx[i][n][1]);
+        else Act<T>::mma(base[n], off_lo, bx[i][n][0], bx[i][n][1]);
+        Act<T>::mma(base[n], off_hi, bx[i][n][2], bx[i][n][3]);
       }
-    }
-    const float s0 = Act<T>::to_float(k.s[0][j]), s1 = Act<T>::to_float(k.s[1][j]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
-      acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
-      acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
-      acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+    for (int m = 0; m < 2; ++m) {
+      float part[NT][4];
+#pragma unroll
+      for (int i = 0; i < B::kWords; ++i) {
+        uint32_t a0[4], a1[4];
+        Act<T>::decode(k.q[2 * m][j * B::kWords + i], a0);
+        Act<T>::decode(k.q[2 * m + 1][j * B::kWords + i], a1);
+        const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (i == 0) Act<T>::mma_from(part[n], lo, bx[i][n][0], bx[i][n][1], base[n]);
+          else Act<T>::mma(part[n], lo, bx[i][n][0], bx[i][n][1]);
+          Act<T>::mma(part[n], hi, bx[i][n][2], bx[i][n][3]);
+        }
+      }
+      const float s0 = Act<T>::to_float(k.s[2 * m][j]), s1 = Act<T>::to_float(k.s[2 * m + 1][j]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[m][n][0] = fmaf(s0, part[n][0], acc[m][n][0]);
+        acc[m][n][1] = fmaf(s0, part[n][1], acc[m][n][1]);
+        acc[m][n][2] = fmaf(s1, part[n][2], acc[m][n][2]);
+        acc[m][n][3] = fmaf(s1, part[n][3], acc[m][n][3]);
+      }
     }
   }
 }
@@ -384,55 +418,103 @@ __device__ __forceinline__ void group_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Blocks of 128 k whose words a warp has in flight.
+constexpr int kRowsDeep = 4;
+constexpr int kRowsSmem = kMvWarps * kRowsDeep * kBlockBytes;
+
+// A place in a warp's run of work: the unit (an expert's strip), the chunk of
+// the expert's rows, the block of K.
+struct RowsWork {
+  int64_t unit;
+  int c0, b;
+};
+
 template <typename T, int GROUP, int NT, bool SWIGLU>
-__global__ void __launch_bounds__(kMvThreads, NT == 1 ? 3 : 2) int4_rows_kernel(const MvParams p) {
+__global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams p) {
   pdl_begin();
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
   constexpr int kTokens = 8 * NT;
-  constexpr int kFeat = SWIGLU ? 8 : 16;  // output features of a strip
-  constexpr int kDeep = NT == 1 ? 2 : 1;  // blocks in flight for a warp
+  constexpr int kFeat = SWIGLU ? 16 : 32;  // output features of a strip
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
+  extern __shared__ __align__(16) uint8_t s_words[];
   __shared__ RowLists s;
-  __shared__ float s_red[kMvWarps][16][kTokens + 1];
+  __shared__ float s_red[kMvWarps][32][kTokens + 1];
   list_rows(s, p);
 
-  const int wk = p.wk;
-  const int groups_in_cta = kMvWarps / wk, group = warp / wk, share = warp % wk;
   const int strips = (p.n_out + kFeat - 1) / kFeat;
   const int blocks = (int)((p.K + 127) / 128);
+  const int64_t units = (int64_t)s.active * strips;
+  // warps that share a strip along K: the number that leaves the longest run of
+  // blocks of any warp shortest, at two blocks' worth for each strip's end
+  int wk = 1;
+  int64_t best = INT64_MAX;
+#pragma unroll 1
+  for (int w = 1; w <= kMvWarps && w <= blocks; w *= 2) {
+    const int64_t teams = (int64_t)gridDim.x * (kMvWarps / w);
+    const int64_t cost = (units + teams - 1) / teams * ((blocks + w - 1) / w + 2);
+    if (cost < best) {
+      best = cost;
+      wk = w;
+    }
+  }
+  const int groups_in_cta = kMvWarps / wk, group = warp / wk, share = warp % wk;
   const int b0 = (int)((int64_t)blocks * share / wk), b1 = (int)((int64_t)blocks * (share + 1) / wk);
   const int kgroups = (int)(p.K / GROUP);
   const T* x = static_cast<const T*>(p.x);
-  const int64_t units = (int64_t)s.active * strips;
   const int64_t stride = (int64_t)gridDim.x * groups_in_cta;
+  // rows of W of this lane: rows g and g + 8 of both tiles (rows past the end
+  // read the last row and are not stored)
+  auto weight_row = [&](int64_t unit, int r) -> int64_t {
+    const int e = s.expert[unit / strips], strip = (int)(unit % strips);
+    int row;
+    if (SWIGLU) row = min(strip * 16 + (r >> 1) * 8 + g, p.n_out - 1) + (r & 1) * p.n_out;
+    else row = min(strip * 32 + r * 8 + g, p.n_out - 1);
+    return (int64_t)e * p.w_rows + row;
+  };
+  auto next = [&](RowsWork& w) -> bool {  // the next block; true: of another unit
+    if (++w.b < b1) return false;
+    w.b = b0;
+    w.c0 += kTokens;
+    if (w.c0 < s.rows[w.unit / strips]) return false;
+    w.c0 = 0;
+    w.unit += stride;
+    return true;
+  };
 
   // neighbouring units on different CTAs: a small launch spreads over the SMs
-  for (int64_t unit = (int64_t)group * gridDim.x + blockIdx.x; unit < units; unit += stride) {
-    const int a = (int)(unit / strips), strip = (int)(unit % strips);
-    const int e = s.expert[a], first = s.first[a], cnt = s.rows[a];
-    // rows of W of this lane: row g and row g + 8 of the strip (rows past the
-    // end read the last row and are not stored)
-    int r0, r1;
-    if (SWIGLU) {
-      r0 = min(strip * 8 + g, p.n_out - 1);
-      r1 = p.n_out + r0;
-    } else {
-      r0 = min(strip * 16 + g, p.n_out - 1);
-      r1 = min(strip * 16 + g + 8, p.n_out - 1);
+  const RowsWork start{(int64_t)group * gridDim.x + blockIdx.x, 0, b0};
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_words) + warp * kRowsDeep * kBlockBytes + lane * 16;
+  RowsWork in = start;  // of the block copied next
+  const uint8_t* w[4] = {};
+  bool moved = true;
+  auto copy_next = [&](int slot) {
+    if (in.unit < units) {
+      if (moved) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = p.w + weight_row(in.unit, r) * (p.K / 2) + t * 4 * kWords;
+      }
+      copy_words<GROUP>(ring + slot * kBlockBytes, w, in.b, kgroups);
+      moved = next(in);
     }
-    const int64_t row0 = (int64_t)e * p.w_rows + r0, row1 = (int64_t)e * p.w_rows + r1;
-    const uint8_t* w0 = p.w + row0 * (p.K / 2) + t * 4 * kWords;
-    const uint8_t* w1 = p.w + row1 * (p.K / 2) + t * 4 * kWords;
-    const T* sc0 = static_cast<const T*>(p.scale) + row0 * kgroups;
-    const T* sc1 = static_cast<const T*>(p.scale) + row1 * kgroups;
-
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRowsDeep - 1; ++i) copy_next(i);
+  int slot = 0;
+  for (int64_t unit = start.unit; unit < units; unit += stride) {
+    const int a = (int)(unit / strips), strip = (int)(unit % strips);
+    const int first = s.first[a], cnt = s.rows[a];
+    const T* sc[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sc[r] = static_cast<const T*>(p.scale) + weight_row(unit, r) * kgroups;
     for (int c0 = 0; c0 < cnt; c0 += kTokens) {
-      float acc[NT][4];
+      float acc[2][NT][4];
       const T* xp[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[0][n][i] = acc[1][n][i] = 0.f;
         const int i = c0 + n * 8 + g;
         xp[n] = nullptr;
         if (i < cnt) {
@@ -441,26 +523,27 @@ __global__ void __launch_bounds__(kMvThreads, NT == 1 ? 3 : 2) int4_rows_kernel(
           xp[n] = x + (int64_t)row * p.K + t * 8 * kWords;
         }
       }
-      for (int b = b0; b < b1; b += kDeep) {
-        Block4<T, GROUP> k[kDeep];
-        uint4 xv[kDeep][NT][4];
+#pragma unroll 1
+      for (int b = b0; b < b1; ++b) {
+        Block4<T, GROUP> k;
+        uint4 xv[NT][4];
+        load_scales<T, GROUP>(k, sc, b, kgroups);
 #pragma unroll
-        for (int u = 0; u < kDeep; ++u) {
-          const int limit = b + u < b1 ? kgroups : 0;  // blocks past the share read as nothing
-          load_block<T, GROUP>(k[u], w0, w1, sc0, sc1, b + u, limit);
+        for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[n], xp[n], b, kgroups);
+        // the slot freed by the last block takes the block kRowsDeep - 1 ahead
+        copy_next(slot == 0 ? kRowsDeep - 1 : slot - 1);
+        copy_wait<kRowsDeep - 1>();
 #pragma unroll
-          for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[u][n], xp[n], b + u, limit);
-        }
-#pragma unroll
-        for (int u = 0; u < kDeep; ++u) multiply_block<T, GROUP, NT>(acc, k[u], xv[u]);
+        for (int r = 0; r < 4; ++r) read_words(ring + slot * kBlockBytes + r * 512, k.q[r]);
+        multiply_block<T, GROUP, NT>(acc, k, xv);
+        slot = slot + 1 == kRowsDeep ? 0 : slot + 1;
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s_red[warp][g][n * 8 + 2 * t] = acc[n][0];
-        s_red[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
-        s_red[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
-        s_red[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
-      }
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s_red[warp][m * 16 + (i >> 1) * 8 + g][n * 8 + 2 * t + (i & 1)] = acc[m][n][i];
       group_barrier(1 + group, 32 * wk);
       // feature f, token n: the shares added in order
       const int tokens = min(kTokens, cnt - c0);
@@ -469,9 +552,10 @@ __global__ void __launch_bounds__(kMvThreads, NT == 1 ? 3 : 2) int4_rows_kernel(
         const int feat = strip * kFeat + f;
         if (feat >= p.n_out) continue;
         float v = 0.f, u = 0.f;
+        const int at_row = SWIGLU ? (f & 8) * 2 + (f & 7) : f;
         for (int k = 0; k < wk; ++k) {
-          v += s_red[group * wk + k][f][n];
-          if (SWIGLU) u += s_red[group * wk + k][f + 8][n];
+          v += s_red[group * wk + k][at_row][n];
+          if (SWIGLU) u += s_red[group * wk + k][at_row + 8][n];
         }
         if (SWIGLU) v = u4::silu_mul(v, u);
         const int place = first + c0 + n;
@@ -482,6 +566,7 @@ __global__ void __launch_bounds__(kMvThreads, NT == 1 ? 3 : 2) int4_rows_kernel(
       group_barrier(1 + group, 32 * wk);
     }
   }
+  copy_wait<0>();
   if (!p.ids) {  // rows behind the last expert's are zero
     const int64_t n0 = (int64_t)s.total * p.n_out, n1 = p.total_rows * p.n_out;
     for (int64_t i = n0 + (int64_t)blockIdx.x * kMvThreads + threadIdx.x; i < n1;
@@ -554,14 +639,11 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
 int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
-  // shares of K: as many as the launch has warps for, each at least two blocks
-  const int64_t blocks = ceil_div(p.K, 128);
-  const int64_t units = ceil_div(p.n_out, SWIGLU ? 8 : 16) * std::min<int64_t>(p.E, rows);
-  const int64_t warps = (int64_t)num_sms() * (NT == 1 ? 3 : 2) * kMvWarps;
-  p.wk = 1;
-  while (p.wk < kMvWarps && 2 * units * p.wk <= warps && blocks >= 4 * p.wk) p.wk *= 2;
-  const int64_t ctas = std::min<int64_t>(ceil_div(units, kMvWarps / p.wk), warps / kMvWarps);
-  MOE_CUDA_TRY(launch_kernel(int4_rows_kernel<T, GROUP, NT, SWIGLU>, dim3((unsigned)ctas), dim3(kMvThreads), 0, st, p));
+  const int64_t units = ceil_div(p.n_out, SWIGLU ? 16 : 32) * std::min<int64_t>(p.E, rows);
+  const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), 2 * num_sms());
+  auto kfn = int4_rows_kernel<T, GROUP, NT, SWIGLU>;
+  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+  MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)ctas), dim3(kMvThreads), kRowsSmem, st, p));
   MOE_LAUNCH_CHECK("int4_rows_kernel");
   return MOE_OK;
 }
