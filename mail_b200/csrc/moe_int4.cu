@@ -1,6 +1,8 @@
 // Experts with 4-bit weights (int4.cuh has the format): quantising and reading
 // back, products grouped by expert for few rows an expert, and the C entry
 // points of the 4-bit operators.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -214,22 +216,23 @@ struct MvParams {
   int x_div;
 };
 
-// A block of 128 k of a lane's four weight rows: rows g and g + 8 of two tiles.
-template <typename T, int GROUP>
+// A block of 128 k of a lane's weight rows: rows g and g + 8 of MT tiles.
+template <typename T, int GROUP, int MT>
 struct Block4 {
   static constexpr int kWords = GROUP / 32;  // 32-bit words a lane holds of a row and group
   static constexpr int kPer = 128 / GROUP;   // groups in the block
-  uint32_t q[4][4];
-  T s[4][kPer];
+  static constexpr int kRows = 2 * MT;
+  static constexpr int kBytes = 512 * kRows;  // of a warp in shared memory
+  uint32_t q[kRows][4];
+  T s[kRows][kPer];
 };
-constexpr int kBlockBytes = 2048;  // of a warp in shared memory: four times 512
 
 // Copies this lane's words of a block to its own 16 bytes for each row in
 // shared memory, asynchronously. Nobody else reads them, so waiting for the
 // copies is all the synchronisation there is. Groups past the end are left out:
 // any words will do, their scales and activations are zero.
-template <int GROUP>
-__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* const (&w)[4], int b, int groups) {
+template <int GROUP, int R>
+__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* const (&w)[R], int b, int groups) {
   constexpr int kPer = 128 / GROUP, kBytes = 16 / kPer;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* const (&
     if (g < groups) {
       const int at = g * (GROUP / 2);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < R; ++r) {
         if constexpr (GROUP == 128)
           asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst + r * 512), "l"(w[r] + at)
                        : "memory");
@@ -262,21 +265,21 @@ __device__ __forceinline__ void read_words(uint32_t src, uint32_t (&v)[4]) {
 }
 
 // The scales of a block; 0 for groups past the end.
-template <typename T, int GROUP>
-__device__ __forceinline__ void load_scales(Block4<T, GROUP>& k, const T* const (&sc)[4], int b, int groups) {
-  using B = Block4<T, GROUP>;
+template <typename T, int GROUP, int MT>
+__device__ __forceinline__ void load_scales(Block4<T, GROUP, MT>& k, const T* const (&sc)[2 * MT], int b, int groups) {
+  using B = Block4<T, GROUP, MT>;
 #pragma unroll
   for (int j = 0; j < B::kPer; ++j) {
     const int g = b * B::kPer + j;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) k.s[r][j] = g < groups ? sc[r][g] : Act<T>::from_float(0.f);
+    for (int r = 0; r < B::kRows; ++r) k.s[r][j] = g < groups ? sc[r][g] : Act<T>::from_float(0.f);
   }
 }
 
 // The activations of eight rows for the block: this lane's row, its words' k.
 template <typename T, int GROUP>
 __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int groups) {
-  using B = Block4<T, GROUP>;
+  using B = Block4<T, GROUP, 1>;
 #pragma unroll
   for (int j = 0; j < B::kPer; ++j)
 #pragma unroll
@@ -288,11 +291,11 @@ __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int 
     }
 }
 
-// acc += the block's products: two tiles of sixteen weight rows by 8 NT tokens.
-template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void multiply_block(float (&acc)[2][NT][4], const Block4<T, GROUP>& k,
+// acc += the block's products: MT tiles of sixteen weight rows by 8 NT tokens.
+template <typename T, int GROUP, int MT, int NT>
+__device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Block4<T, GROUP, MT>& k,
                                                const uint4 (&x)[NT][4]) {
-  using B = Block4<T, GROUP>;
+  using B = Block4<T, GROUP, MT>;
   constexpr uint32_t off_lo[4] = {Act<T>::kOffset[0], Act<T>::kOffset[0], Act<T>::kOffset[1], Act<T>::kOffset[1]};
   constexpr uint32_t off_hi[4] = {Act<T>::kOffset[2], Act<T>::kOffset[2], Act<T>::kOffset[3], Act<T>::kOffset[3]};
 #pragma unroll
@@ -309,7 +312,7 @@ __device__ __forceinline__ void multiply_block(float (&acc)[2][NT][4], const Blo
         Act<T>::mma(base[n], off_hi, bx[i][n][2], bx[i][n][3]);
       }
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    for (int m = 0; m < MT; ++m) {
       float part[NT][4];
 #pragma unroll
       for (int i = 0; i < B::kWords; ++i) {
@@ -420,7 +423,7 @@ __device__ __forceinline__ void group_barrier(int id, int threads) {
 
 // Blocks of 128 k whose words a warp has in flight.
 constexpr int kRowsDeep = 4;
-constexpr int kRowsSmem = kMvWarps * kRowsDeep * kBlockBytes;
+constexpr int kRowsSmem = kMvWarps * kRowsDeep * 2048;
 
 // A place in a warp's run of work: the unit (an expert's strip), the chunk of
 // the expert's rows, the block of K.
@@ -435,6 +438,8 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
   constexpr int kTokens = 8 * NT;
   constexpr int kFeat = SWIGLU ? 16 : 32;  // output features of a strip
+  using B = Block4<T, GROUP, 2>;
+  constexpr int kBlockBytes = B::kBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   extern __shared__ __align__(16) uint8_t s_words[];
@@ -525,9 +530,9 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
       }
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
-        Block4<T, GROUP> k;
+        B k;
         uint4 xv[NT][4];
-        load_scales<T, GROUP>(k, sc, b, kgroups);
+        load_scales<T, GROUP, 2>(k, sc, b, kgroups);
 #pragma unroll
         for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[n], xp[n], b, kgroups);
         // the slot freed by the last block takes the block kRowsDeep - 1 ahead
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
         copy_wait<kRowsDeep - 1>();
 #pragma unroll
         for (int r = 0; r < 4; ++r) read_words(ring + slot * kBlockBytes + r * 512, k.q[r]);
-        multiply_block<T, GROUP, NT>(acc, k, xv);
+        multiply_block<T, GROUP, 2, NT>(acc, k, xv);
         slot = slot + 1 == kRowsDeep ? 0 : slot + 1;
       }
 #pragma unroll
@@ -575,6 +580,160 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
       else static_cast<uint16_t*>(p.out)[i] = 0;
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// The down projection and the combine of a decode batch in one launch:
+//   y[t, c] = sum_j weight[t, j] sum_k h[slot (t, j), k] W2[id(t, j), c, k]
+//
+// A cluster of CTAs takes a strip of sixteen output features and every expert
+// that has rows; its warps share the blocks of all experts' rows evenly and add
+// their tiles, times the routing weights, to sums of their own for each token.
+// Those are added over the warps of a CTA, then over the CTAs of the cluster
+// through distributed shared memory, always in the same order, and rounded
+// once: no atomics, no buffer of rows, and no third launch. The lists and the
+// first words do not depend on h, so they are read before the wait for the
+// gate_up launch (which itself has waited for whatever wrote ids and weights).
+constexpr int kDownTokens = 32;
+constexpr int kDownSlots = 256;
+constexpr int kDownDeep = 6;
+
+struct DownParams {
+  const void* h;         // [slots, K]
+  const uint8_t* w;      // [E, n_out, K / 2]
+  const void* scale;
+  const float* weights;  // [slots]
+  const int32_t* ids;    // [slots]
+  void* y;               // [tokens, n_out]
+  int64_t K;
+  int n_out, E, tokens, top_k, slots, cluster;
+};
+
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownParams p) {
+  constexpr int kWords = GROUP / 32;
+  using B = Block4<T, GROUP, 1>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  extern __shared__ __align__(16) uint8_t s_words[];
+  __shared__ RowLists s;
+  __shared__ int s_tile_expert[kDownSlots], s_tile_first[kDownSlots], s_tile_rows[kDownSlots], s_tiles;
+  __shared__ float s_sum[kMvWarps][kDownTokens][17];
+  __shared__ int64_t warp_sums[32];
+
+  MvParams lists{};
+  lists.ids = p.ids;
+  lists.slots = p.slots;
+  lists.E = p.E;
+  list_rows(s, lists);
+  {
+    // tiles of up to eight rows of an expert (an expert for each thread at most)
+    const int rows = tid < s.active ? s.rows[tid] : 0;
+    const int64_t mine = (rows + 7) / 8;
+    const int64_t incl = block_inclusive_scan<int64_t>(mine, warp_sums);
+    for (int i = 0; i < (int)mine; ++i) {
+      const int at = (int)(incl - mine) + i;
+      s_tile_expert[at] = s.expert[tid];
+      s_tile_first[at] = s.first[tid] + 8 * i;
+      s_tile_rows[at] = min(8, rows - 8 * i);
+    }
+    if (tid == kMvThreads - 1) s_tiles = (int)incl;
+  }
+  for (int i = lane; i < p.tokens * 17; i += 32) s_sum[warp][i / 17][i % 17] = 0.f;
+  __syncthreads();
+
+  const int rank = blockIdx.x % p.cluster, strip = blockIdx.x / p.cluster;
+  const int blocks = (int)((p.K + 127) / 128), kgroups = (int)(p.K / GROUP);
+  const int64_t work = (int64_t)s_tiles * blocks;
+  const int me = rank * kMvWarps + warp, all = p.cluster * kMvWarps;
+  const int64_t lo = work * me / all, hi = work * (me + 1) / all;
+  const int r0 = min(strip * 16 + g, p.n_out - 1), r1 = min(strip * 16 + g + 8, p.n_out - 1);
+
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_words) + warp * kDownDeep * B::kBytes + lane * 16;
+  int64_t in = lo;
+  int in_tile = (int)(lo / blocks), in_b = (int)(lo % blocks);
+  const uint8_t* w[2] = {};
+  bool moved = true;
+  auto copy_next = [&](int slot) {
+    if (in < hi) {
+      if (moved) {
+        const int64_t base = (int64_t)s_tile_expert[in_tile] * p.n_out;
+        w[0] = p.w + (base + r0) * (p.K / 2) + t * 4 * kWords;
+        w[1] = p.w + (base + r1) * (p.K / 2) + t * 4 * kWords;
+      }
+      copy_words<GROUP, 2>(ring + slot * B::kBytes, w, in_b, kgroups);
+      ++in;
+      moved = ++in_b == blocks;
+      if (moved) {
+        in_b = 0;
+        ++in_tile;
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kDownDeep - 1; ++i) copy_next(i);
+  pdl_begin();  // h
+
+  int slot = 0;
+  int64_t at = lo;
+  int tile = (int)(lo / blocks), b = (int)(lo % blocks);
+  while (at < hi) {
+    const int64_t base = (int64_t)s_tile_expert[tile] * p.n_out;
+    const T* sc[2] = {static_cast<const T*>(p.scale) + (base + r0) * kgroups,
+                      static_cast<const T*>(p.scale) + (base + r1) * kgroups};
+    const int rows = s_tile_rows[tile], first = s_tile_first[tile];
+    const T* xp = g < rows ? static_cast<const T*>(p.h) + (int64_t)s.list[first + g] * p.K + t * 8 * kWords : nullptr;
+    const int end = (int)min((int64_t)blocks, b + (hi - at));
+    float acc[1][1][4] = {};
+    at += end - b;
+#pragma unroll 1
+    for (; b < end; ++b) {
+      B k;
+      uint4 xv[1][4];
+      load_scales<T, GROUP, 1>(k, sc, b, kgroups);
+      load_acts<T, GROUP>(xv[0], xp, b, kgroups);
+      copy_next(slot == 0 ? kDownDeep - 1 : slot - 1);
+      copy_wait<kDownDeep - 1>();
+      read_words(ring + slot * B::kBytes, k.q[0]);
+      read_words(ring + slot * B::kBytes + 512, k.q[1]);
+      multiply_block<T, GROUP, 1, 1>(acc, k, xv);
+      slot = slot + 1 == kDownDeep ? 0 : slot + 1;
+    }
+    // column by column: two rows of a tile may belong to one token
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (n < rows && t == n / 2) {
+        const int sl = s.list[first + n];
+        const float weight = p.weights[sl];
+        float* sum = s_sum[warp][sl / p.top_k];
+        sum[g] = fmaf(weight, acc[0][0][n & 1], sum[g]);
+        sum[g + 8] = fmaf(weight, acc[0][0][2 + (n & 1)], sum[g + 8]);
+      }
+      __syncwarp();
+    }
+    b = 0;
+    ++tile;
+  }
+  copy_wait<0>();
+  __syncthreads();
+  // this CTA's sums, into the first warp's place
+  for (int i = tid; i < p.tokens * 16; i += kMvThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMvWarps; ++k) v += s_sum[k][i >> 4][i & 15];
+    s_sum[0][i >> 4][i & 15] = v;
+  }
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  if (rank == 0) {
+    for (int i = tid; i < p.tokens * 16; i += kMvThreads) {
+      const int tok = i >> 4, f = i & 15;
+      float v = s_sum[0][tok][f];
+      for (int c = 1; c < p.cluster; ++c) v += *cluster.map_shared_rank(&s_sum[0][tok][f], c);
+      if (strip * 16 + f < p.n_out) static_cast<T*>(p.y)[(int64_t)tok * p.n_out + strip * 16 + f] = Act<T>::from_float(v);
+    }
+  }
+  cluster.sync();  // no CTA leaves while its sums are read
 }
 
 // y[t] = sum_j weight[t, j] * o[row of slot (t, j)], slots in order; a slot
@@ -654,6 +813,47 @@ int launch_rows_group(const MvParams& p, int64_t rows, cudaStream_t st) {
   return launch_rows_nt<T, GROUP, 2, SWIGLU>(p, rows, st);
 }
 
+template <typename T, int GROUP>
+int launch_down(DownParams p, cudaStream_t st) {
+  // CTAs of a cluster: as many (1, 2, 4 or 8) as two a SM leave room for
+  const int strips = (int)ceil_div(p.n_out, 16);
+  p.cluster = 1;
+  while (p.cluster < 8 && 2 * p.cluster * strips <= 2 * num_sms()) p.cluster *= 2;
+  auto kfn = int4_down_kernel<T, GROUP>;
+  const int smem = kMvWarps * kDownDeep * Block4<T, GROUP, 1>::kBytes;
+  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3((unsigned)(strips * p.cluster));
+  cfg.blockDim = dim3(kMvThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.numAttrs = 1;
+  if (pdl_enabled()) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kfn, p));
+  MOE_LAUNCH_CHECK("int4_down_kernel");
+  return MOE_OK;
+}
+
+int launch_down_any(const DownParams& p, int dtype, int group, cudaStream_t st) {
+  if (dtype == MOE_BF16) {
+    if (group == 128) return launch_down<__nv_bfloat16, 128>(p, st);
+    if (group == 64) return launch_down<__nv_bfloat16, 64>(p, st);
+    return launch_down<__nv_bfloat16, 32>(p, st);
+  }
+  if (group == 128) return launch_down<__half, 128>(p, st);
+  if (group == 64) return launch_down<__half, 64>(p, st);
+  return launch_down<__half, 32>(p, st);
+}
+
 // Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM).
 constexpr int64_t kRowsPerExpert = 16;
 bool use_gemm(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
@@ -687,6 +887,7 @@ struct LayerWs {
   size_t xp, h, o, align, sorted, slot_pos, gs, poff, table, align_bytes, bytes;
   bool gemm;    // tensor-core tiles
   bool direct;  // the top-k ids are read by the product kernels themselves
+  bool down;    // the down projection and the combine in one launch
 };
 LayerWs layer_ws(int64_t T, int64_t H, int64_t I, int E, int k) {
   LayerWs w{};
@@ -699,9 +900,10 @@ LayerWs layer_ws(int64_t T, int64_t H, int64_t I, int E, int k) {
   };
   w.gemm = use_gemm(S, std::max(H, I), std::max(H, 2 * I), E);
   w.direct = !w.gemm && S <= kMaxSlots;
+  w.down = w.direct && S <= kDownSlots && T <= kDownTokens;
   w.xp = take(w.gemm ? (size_t)S * H * 2 : 0);
   w.h = take((size_t)S * I * 2);
-  w.o = take((size_t)S * H * sizeof(float));
+  w.o = take(w.down ? 0 : (size_t)S * H * sizeof(float));
   if (!w.direct) {
     w.align_bytes = moe_align_workspace_size(T, k, E, 1);
     w.align = take(w.align_bytes);
@@ -867,6 +1069,22 @@ extern "C" int moe_fused_experts_int4(const void* x, int dtype, int64_t num_toke
   p.n_out = (int)inter;
   p.w_rows = (int)(2 * inter);
   MOE_TRY(launch_grouped<true>(p, dtype, group_size, w.gemm, st));
+  if (w.down) {
+    DownParams d{};
+    d.h = ws + w.h;
+    d.w = w2;
+    d.scale = w2_scale;
+    d.weights = topk_weights;
+    d.ids = topk_ids;
+    d.y = y;
+    d.K = inter;
+    d.n_out = (int)hidden;
+    d.E = num_experts;
+    d.tokens = (int)num_tokens;
+    d.top_k = top_k;
+    d.slots = (int)S;
+    return launch_down_any(d, dtype, group_size, st);
+  }
   p.x = ws + w.h;
   p.w = w2;
   p.scale = w2_scale;

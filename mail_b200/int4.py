@@ -17,28 +17,43 @@ tensors' device; there is no CPU or PyTorch fallback.
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
-from .moe import _check_shapes, _code, _require_cuda, _stream, _workspace, kmajor
+from .moe import _check_shapes, _require_cuda, _stream, kmajor
 
 GROUP_SIZES = (32, 64, 128)
 _ACT = (torch.bfloat16, torch.float16)
+_CODES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _on(dev: torch.device):
-    """Makes `dev` current for the launches inside."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """The C call with `args` and the current stream of `dev`, with `dev` current.
+    (A decode step is a few microseconds of kernels, so the host's share of a
+    call counts: the stream is read as an integer, without a Stream object.)"""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
 
 
 def _one_device(name: str, *ts: torch.Tensor) -> torch.device:
-    _require_cuda(*ts)
     dev = ts[0].device
-    if any(t.device != dev for t in ts):
-        raise ValueError(f"{name}: all tensors must be on one device")
+    for t in ts:
+        if not t.is_cuda:
+            _require_cuda(t)
+        if t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on one device")
     return dev
+
+
+def _kmajor(w: torch.Tensor) -> torch.Tensor:
+    """w itself where its storage is K-major (the same first byte as the [E, N, K / 2]
+    view's), a K-major copy otherwise."""
+    E, K2, N = w.shape
+    s0, s1, s2 = w.stride()
+    return w if s1 == 1 and s2 == K2 and (s0 == K2 * N or E == 1) else kmajor(w)
 
 
 def _check_group(name: str, K: int, group_size: int) -> None:
@@ -66,9 +81,8 @@ def quant_int4_groups(w: torch.Tensor, group_size: int = 128, scale_dtype: torch
     w = w.contiguous()
     q = torch.empty((R, C // 2), dtype=torch.uint8, device=w.device)
     s = torch.empty((R, C // group_size), dtype=scale_dtype, device=w.device)
-    with _on(w.device):
-        _lib.call("moe_quant_int4_groups", w.data_ptr(), _code(w), R, C, group_size, q.data_ptr(), s.data_ptr(),
-                  _code(s), _stream(w.device))
+    _launch(w.device, "moe_quant_int4_groups", w.data_ptr(), _CODES[w.dtype], R, C, group_size, q.data_ptr(),
+            s.data_ptr(), _CODES[scale_dtype])
     return q, s
 
 
@@ -88,9 +102,8 @@ def dequant_int4_groups(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype
     if out.dtype not in (*_ACT, torch.float32):
         raise TypeError(f"dequant_int4_groups: dtype must be bf16, fp16 or fp32, not {out.dtype}")
     q, scale = q.contiguous(), scale.contiguous()
-    with _on(dev):
-        _lib.call("moe_dequant_int4_groups", q.data_ptr(), scale.data_ptr(), _code(scale), R, C, group_size,
-                  out.data_ptr(), _code(out), _stream(dev))
+    _launch(dev, "moe_dequant_int4_groups", q.data_ptr(), scale.data_ptr(), _CODES[scale.dtype], R, C, group_size,
+            out.data_ptr(), _CODES[out.dtype])
     return out
 
 
@@ -162,11 +175,10 @@ def _grouped_impl(x, w, scale, group_sizes):
     group_size = _check_weight(name, x.dtype, w, scale, K)
     E, _, N = w.shape
     gs = _counts(name, group_sizes, E)
-    x, wk, scale = x.contiguous(), kmajor(w), scale.contiguous()
+    x, wk, scale = x.contiguous(), _kmajor(w), scale.contiguous()
     out = torch.empty((T, N), dtype=x.dtype, device=dev)
-    with _on(dev):
-        _lib.call("moe_grouped_matmul_int4", x.data_ptr(), _code(x), T, K, wk.data_ptr(), scale.data_ptr(),
-                  group_size, E, N, gs.data_ptr(), _code(gs), out.data_ptr(), _stream(dev))
+    _launch(dev, "moe_grouped_matmul_int4", x.data_ptr(), _CODES[x.dtype], T, K, wk.data_ptr(), scale.data_ptr(),
+            group_size, E, N, gs.data_ptr(), _lib.I32 if gs.dtype == torch.int32 else _lib.I64, out.data_ptr())
     return out
 
 
@@ -182,7 +194,7 @@ def _layer_weights(x, w13, w2, w13_scale, w2_scale):
     group = _check_weight(name, x.dtype, w13, w13_scale, H)
     if _check_weight(name, x.dtype, w2, w2_scale, two_i // 2) != group:
         raise ValueError(f"{name}: w13 and w2 must share a group size")
-    return E, H, two_i // 2, group, kmajor(w13), w13_scale.contiguous(), kmajor(w2), w2_scale.contiguous()
+    return E, H, two_i // 2, group, _kmajor(w13), w13_scale.contiguous(), _kmajor(w2), w2_scale.contiguous()
 
 
 def fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
@@ -195,11 +207,11 @@ def fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
     ids = topk_ids.to(torch.int32).contiguous()
     T, k = ids.shape
     y = torch.empty((T, H), dtype=x.dtype, device=dev)
-    ws = _workspace(_lib.query("moe_fused_experts_int4_workspace_size", T, H, inter, E, k), dev)
-    with _on(dev):
-        _lib.call("moe_fused_experts_int4", x.data_ptr(), _code(x), T, H, a.data_ptr(), sa.data_ptr(), b.data_ptr(),
-                  sb.data_ptr(), group, E, inter, wts.data_ptr(), ids.data_ptr(), k, y.data_ptr(), ws.data_ptr(),
-                  ws.numel(), _stream(dev))
+    size = _lib.query("moe_fused_experts_int4_workspace_size", T, H, inter, E, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _launch(dev, "moe_fused_experts_int4", x.data_ptr(), _CODES[x.dtype], T, H, a.data_ptr(), sa.data_ptr(),
+            b.data_ptr(), sb.data_ptr(), group, E, inter, wts.data_ptr(), ids.data_ptr(), k, y.data_ptr(),
+            ws.data_ptr(), size)
     return y
 
 
@@ -213,11 +225,11 @@ def fused_mlp(x, w13, w2, group_sizes, w13_scale, w2_scale):
     gs = _counts("fused_moe_mlp", group_sizes, E)
     T = x.shape[0]
     out = torch.empty((T, H), dtype=x.dtype, device=dev)
-    ws = _workspace(_lib.query("moe_fused_mlp_int4_workspace_size", T, inter, E), dev)
-    with _on(dev):
-        _lib.call("moe_fused_mlp_int4", x.data_ptr(), _code(x), T, H, a.data_ptr(), sa.data_ptr(), b.data_ptr(),
-                  sb.data_ptr(), group, E, inter, gs.data_ptr(), _code(gs), out.data_ptr(), ws.data_ptr(), ws.numel(),
-                  _stream(dev))
+    size = _lib.query("moe_fused_mlp_int4_workspace_size", T, inter, E)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _launch(dev, "moe_fused_mlp_int4", x.data_ptr(), _CODES[x.dtype], T, H, a.data_ptr(), sa.data_ptr(), b.data_ptr(),
+            sb.data_ptr(), group, E, inter, gs.data_ptr(), _lib.I32 if gs.dtype == torch.int32 else _lib.I64,
+            out.data_ptr(), ws.data_ptr(), size)
     return out
 
 
