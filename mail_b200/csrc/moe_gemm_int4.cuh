@@ -295,7 +295,6 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
     int item = blockIdx.x, kb = 0, h0 = 0, h1 = 0, h2 = 0, row = 0;
     uint32_t bytes = 0, phase = 0;
     auto start = [&]() {
-      if (item >= total) return;
       const Int4Item it = int4_item(item, s_cum, s_off, E, p.nf);
       row = (int)it.row;
       int left = (it.rows + 15) & ~15;
@@ -310,31 +309,41 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
       h2 = take(true);
       bytes = (uint32_t)(h0 + h1 + h2) * ROW_BYTES;
     };
-    auto box = [&](int h) { return &maps.x[31 - __clz(h) - 4]; };
-    start();
-    bool ok = true;
+    auto box = [&](int h) { return &maps.x[h ? 31 - __clz(h) - 4 : 0]; };
+    auto x_load = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y) {
+      asm volatile(
+          "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+              dst),
+          "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(ptx::smem_u32(bar))
+          : "memory");
+    };
+    const bool issuer = ptx::elect_one();
+    bool ok = true, ready = false;
     int st = 0, filled = 0;
     while (item < total) {
-      ok = int4_wait<20>(ptx::mbar_test_wait(&sm.empty[st], phase ^ 1), &sm.empty[st], phase ^ 1, abort_flag);
+      start();
+      const CUtensorMap *m0 = box(h0), *m1 = box(h1), *m2 = box(h2);
+      for (kb = 0; kb < nkb; ++kb) {
+        uint64_t* const full = &sm.full[st];
+        const uint32_t dst = ptx::smem_u32(sX + st * Sh::kXBytes);
+        ok = int4_wait<20>(ready, &sm.empty[st], phase ^ 1, abort_flag);
+        if (!ok) break;
+        if (++st == kStages) {
+          st = 0;
+          phase ^= 1;
+        }
+        ready = ptx::mbar_test_wait(&sm.empty[st], phase ^ 1);
+        if (issuer) {
+          ptx::mbar_arrive_expect_tx(full, bytes);
+          x_load(dst, m0, full, kb * Q4_KB, row);
+        }
+        if (h1 && issuer) x_load(dst + h0 * ROW_BYTES, m1, full, kb * Q4_KB, row + h0);
+        if (h2 && issuer) x_load(dst + (h0 + h1) * ROW_BYTES, m2, full, kb * Q4_KB, row + h0 + h1);
+        __syncwarp();
+        filled = min(filled + 1, kStages);
+      }
       if (!ok) break;
-      if (ptx::elect_one()) {
-        uint8_t* dst = sX + st * Sh::kXBytes;
-        ptx::mbar_arrive_expect_tx(&sm.full[st], bytes);
-        ptx::tma_load_2d(dst, box(h0), &sm.full[st], kb * Q4_KB, row);
-        if (h1) ptx::tma_load_2d(dst + h0 * ROW_BYTES, box(h1), &sm.full[st], kb * Q4_KB, row + h0);
-        if (h2) ptx::tma_load_2d(dst + (h0 + h1) * ROW_BYTES, box(h2), &sm.full[st], kb * Q4_KB, row + h0 + h1);
-      }
-      __syncwarp();
-      if (++st == kStages) {
-        st = 0;
-        phase ^= 1;
-      }
-      filled = min(filled + 1, kStages);
-      if (++kb == nkb) {
-        kb = 0;
-        item += gridDim.x;
-        start();
-      }
+      item += gridDim.x;
     }
     if (!ok && lane == 0) {
       raise_device_error(1);

@@ -322,7 +322,7 @@ __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Bl
         const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if (i == 0) Act<T>::mma_from(part[n], lo, bx[i][n][0], bx[i][n][1], base[n]);
+          if (i == 0) Act<T>::mma_first(part[n], lo, bx[i][n][0], bx[i][n][1]);
           else Act<T>::mma(part[n], lo, bx[i][n][0], bx[i][n][1]);
           Act<T>::mma(part[n], hi, bx[i][n][2], bx[i][n][3]);
         }
@@ -330,10 +330,10 @@ __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Bl
       const float s0 = Act<T>::to_float(k.s[2 * m][j]), s1 = Act<T>::to_float(k.s[2 * m + 1][j]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[m][n][0] = fmaf(s0, part[n][0], acc[m][n][0]);
-        acc[m][n][1] = fmaf(s0, part[n][1], acc[m][n][1]);
-        acc[m][n][2] = fmaf(s1, part[n][2], acc[m][n][2]);
-        acc[m][n][3] = fmaf(s1, part[n][3], acc[m][n][3]);
+        acc[m][n][0] = fmaf(s0, part[n][0] + base[n][0], acc[m][n][0]);
+        acc[m][n][1] = fmaf(s0, part[n][1] + base[n][1], acc[m][n][1]);
+        acc[m][n][2] = fmaf(s1, part[n][2] + base[n][2], acc[m][n][2]);
+        acc[m][n][3] = fmaf(s1, part[n][3] + base[n][3], acc[m][n][3]);
       }
     }
   }
