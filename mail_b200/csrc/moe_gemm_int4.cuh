@@ -43,22 +43,25 @@ constexpr size_t Q4_MAX_SMEM = 227 * 1024;
 // narrow ones, with more blocks in flight, where the weights bound the launch.
 //
 // Set s of the decoding warps takes every kSets-th MMA block (64 k) and writes
-// it to stages s and s + kSets in turn: it decodes one while the other
-// multiplies, and it waits for no use of a stage but the one after its own
-// last. (A wait on a barrier's parity cannot tell a use from the use two before
-// it; a set that shared stages could overtake a slower one.) The words' slots
-// are shared: a set that has written block kb knows the blocks up to
-// kb - kStages - kSets multiplied, so with kMinRaw slots or more the use before
-// the one that it waits for is over.
+// it to the stages s, s + kSets, .. in turn, so it waits for no use of a stage
+// but the one after its own last. (A wait on a barrier's parity cannot tell a use
+// from the use two before it; a set that shared stages could overtake a slower
+// one.) The words' slots are shared, kRawStep by kRawStep between kMinRaw and
+// kMaxRaw of them, so that the same holds there: three sets know the blocks of
+// words up to five before the next one multiplied; four sets come to every
+// second block, and an even number of slots makes a slot's last use their own.
+// Narrow tiles have two stages for each set: it decodes one while the other
+// multiplies. Wide ones multiply longer than they decode, and four sets with a
+// stage each keep up.
 template <bool NARROW>
 struct Int4Shape {
   static constexpr int kRows = NARROW ? 64 : 256;  // rows of x of a tile at most (UMMA N)
-  static constexpr int kSets = NARROW ? 3 : 2;
-  static constexpr int kStages = 2 * kSets;        // MMA blocks of decoded weights and rows of x
+  static constexpr int kSets = NARROW ? 3 : 4;
+  static constexpr int kStages = NARROW ? 6 : 4;   // MMA blocks of decoded weights and rows of x
   static constexpr int kMaxRaw = NARROW ? 9 : 4;   // blocks (128 k) of words and scales
-  static constexpr int kMinRaw = NARROW ? 6 : 2;
+  static constexpr int kMinRaw = NARROW ? 6 : 2, kRawStep = NARROW ? 1 : 2;
   static constexpr uint32_t kXBytes = kRows * ROW_BYTES;
-  static constexpr int kThreads = NARROW ? 640 : 512;
+  static constexpr int kThreads = 32 * (8 + 4 * kSets);
 };
 // Narrow tiles up to this many rows an expert on average.
 constexpr int64_t kInt4NarrowRows = 48;
@@ -173,8 +176,8 @@ __device__ __forceinline__ uint4 decode_word(uint32_t w, uint32_t s2) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Waits at once if `ready` (an earlier mbar_test_wait of the same phase) is
-// false. The same answer for the whole warp.
+// Waits at once if `ready` (an earlier look at the same phase found it
+// complete). The same answer for the whole warp.
 template <int NS>
 __device__ __forceinline__ bool int4_wait(bool ready, uint64_t* bar, uint32_t parity, volatile int* abort) {
   if (__all_sync(0xffffffffu, ready)) return true;
@@ -201,17 +204,25 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
   volatile int* abort_flag = &sm.abort_flag;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // warps 1, 5, 9, .. (one scheduler): MMA issue, rows of x, words, a quarter of
-  // the epilogue; warps 0, 2, 3: the other quarters; then the decoding warps
-  // and, last, the scales
-  enum { kIssue, kRowsIn, kWordsIn, kScalesIn, kEpilogue, kDecode, kIdle };
-  const int sub = warp & 3, level = warp >> 2;
-  const int decoder = (level - 1) * 3 + (sub == 0 ? 0 : sub - 1);
-  const int role = sub == 1 ? (level == 0 ? kIssue : level == 1 ? kRowsIn : level == 2 ? kWordsIn
-                                                 : level == 3 ? kEpilogue : kScalesIn)
-                            : (level == 0 ? kEpilogue : decoder < 4 * kSets ? kDecode
-                                                      : NARROW ? kIdle : kScalesIn);
-  static_assert(Sh::kThreads == (NARROW ? 20 : 16) * 32 && 4 * kSets == (NARROW ? 12 : 8), "one scales warp");
+  // Wide: warps 0..3 epilogue, 4..7 issue and loads, the others decode, four on
+  // each scheduler. Narrow: issue, the loads and a quarter of the epilogue have
+  // the scheduler of warps 1, 5, 9, .. to themselves, since there the MMAs of a
+  // block take no longer than their issue (layer of 256 experts at 1024 tokens:
+  // 2577 against 2693 us; the wide shape that way: 779 against 741 us).
+  enum { kIssue, kRowsIn, kWordsIn, kScalesIn, kEpilogue, kDecode };
+  int role, decoder;
+  if constexpr (NARROW) {
+    const int sub = warp & 3, level = warp >> 2;
+    decoder = (level - 1) * 3 + (sub == 0 ? 0 : sub - 1);
+    role = sub != 1 ? (level == 0 ? kEpilogue : kDecode)
+                    : level == 0 ? kIssue : level == 1 ? kRowsIn : level == 2 ? kWordsIn
+                                                     : level == 3 ? kEpilogue : kScalesIn;
+    static_assert(!NARROW || 4 * kSets == 12, "decoding warps on three schedulers");
+  } else {
+    decoder = warp - 8;
+    role = warp < 4 ? kEpilogue : warp == 4 ? kIssue : warp == 5 ? kRowsIn : warp == 6 ? kWordsIn
+                                             : warp == 7 ? kScalesIn : kDecode;
+  }
   const int E = p.E;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.raw; ++i) {
@@ -408,7 +419,8 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
     // one's MMAs are issued. A block of four MMAs with few columns takes 157
     // cycles on the tensor cores; issued from a single lane with the stage in
     // a register it took 530, this way it takes 190.
-    const uint64_t a_desc = ptx::smem_desc_k128(ptx::smem_u32(sA)), x_desc = ptx::smem_desc_k128(ptx::smem_u32(sX));
+    const uint32_t a_desc = ptx::smem_desc_k128_lo(ptx::smem_u32(sA));
+    const uint32_t x_desc = ptx::smem_desc_k128_lo(ptx::smem_u32(sX));
     const bool issuer = ptx::elect_one();
     int item = blockIdx.x, n = 0, kb = 0;
     uint32_t phase = 0, idesc = 0, d = 0;
@@ -430,11 +442,10 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
         ptx::tc_fence_after();
         ready = ptx::mbar_test_wait(&sm.full[(st + 1) % kStages], st + 1 == kStages ? phase ^ 1 : phase);
         if (issuer) {
-          const uint64_t ad = a_desc + (uint64_t)(st * (Q4_A_BYTES >> 4));
-          const uint64_t xd = x_desc + (uint64_t)(st * (Sh::kXBytes >> 4));
+          const uint32_t ad = a_desc + st * (Q4_A_BYTES >> 4), xd = x_desc + st * (Sh::kXBytes >> 4);
 #pragma unroll
           for (int k = 0; k < ROW_BYTES / 32; ++k)
-            ptx::umma<0>(d, ad + 2 * k, xd + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            ptx::umma_k128(d, ad + 2 * k, xd + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           ptx::umma_commit(&sm.empty[st]);
         }
         __syncwarp();
@@ -644,11 +655,10 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
         // waited for, and the slot's next words came in under them
         ptx::mbar_arrive(&sm.raw_empty[slot]);
       }
-      if (stage >= kSets) {
+      stage += kSets;
+      if (stage >= kStages) {
         stage = set;
         phase ^= 1;
-      } else {
-        stage += kSets;
       }
       slot += ((int)kb + kSets) / 2 - (int)kb / 2;
       if (slot >= p.raw) {
@@ -681,7 +691,7 @@ template <typename T, int GROUP, bool SWIGLU, bool NARROW>
 int launch_int4_gemm(const Int4Maps& maps, Int4Params p, int64_t rows_hit, cudaStream_t st) {
   using Sh = Int4Shape<NARROW>;
   p.raw = Sh::kMaxRaw;
-  while (p.raw > Sh::kMinRaw && int4_gemm_smem<NARROW>(p.raw, GROUP, p.E) > Q4_MAX_SMEM) --p.raw;
+  while (p.raw > Sh::kMinRaw && int4_gemm_smem<NARROW>(p.raw, GROUP, p.E) > Q4_MAX_SMEM) p.raw -= Sh::kRawStep;
   const size_t smem = int4_gemm_smem<NARROW>(p.raw, GROUP, p.E);
   auto kfn = int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>;
   MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
