@@ -20,10 +20,24 @@ __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinter
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
 // (v & mask) | bits in one instruction; written in C the two constants cost two.
-__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t bits) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "r"(bits));
   return r;
+}
+
+// The exponents that decode() sets, kept in registers: as constants they would
+// be moved into one for each use.
+struct Exponents {
+  uint32_t first, rest;
+};
+template <uint32_t FIRST, uint32_t REST>
+__device__ __forceinline__ Exponents held_exponents() {
+  Exponents e;
+  asm volatile("mov.b32 %0, %1;" : "=r"(e.first) : "n"(FIRST));
+  asm volatile("mov.b32 %0, %1;" : "=r"(e.rest) : "n"(REST));
+  return e;
 }
 
 // The 16-bit activation types.
@@ -37,11 +51,12 @@ struct Act<__nv_bfloat16> {
   // the highest four. Left as it is, M costs no instruction for each weight;
   // kOffset, -(M + 8), multiplied by the same
   // activations, takes it out of the sums.
-  static __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4]) {
-    p[0] = and_or(w, 0x000f000fu, 0x43004300u);
-    p[1] = and_or(w >> 1, 0x00780078u, 0x41804180u);
-    p[2] = and_or(w >> 5, 0x00780078u, 0x41804180u);
-    p[3] = and_or(w >> 9, 0x00780078u, 0x41804180u);
+  static __device__ __forceinline__ Exponents exponents() { return held_exponents<0x43004300u, 0x41804180u>(); }
+  static __device__ __forceinline__ void decode(uint32_t w, const Exponents& e, uint32_t (&p)[4]) {
+    p[0] = and_or<0x000f000fu>(w, e.first);
+    p[1] = and_or<0x00780078u>(w >> 1, e.rest);
+    p[2] = and_or<0x00780078u>(w >> 5, e.rest);
+    p[3] = and_or<0x00780078u>(w >> 9, e.rest);
   }
   static constexpr uint32_t kOffset[4] = {0xc308c308u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};  // -136, -24, ..
   static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -70,11 +85,12 @@ template <>
 struct Act<__half> {
   // M + q: ten mantissa bits take (k1, k5) as it stands, with M = 64; the other
   // pairs shifted to the highest four, with M = 16
-  static __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4]) {
-    p[0] = and_or(w << 6, 0x03c003c0u, 0x4c004c00u);
-    p[1] = and_or(w, 0x00f000f0u, 0x54005400u);
-    p[2] = and_or(w >> 2, 0x03c003c0u, 0x4c004c00u);
-    p[3] = and_or(w >> 6, 0x03c003c0u, 0x4c004c00u);
+  static __device__ __forceinline__ Exponents exponents() { return held_exponents<0x54005400u, 0x4c004c00u>(); }
+  static __device__ __forceinline__ void decode(uint32_t w, const Exponents& e, uint32_t (&p)[4]) {
+    p[0] = and_or<0x03c003c0u>(w << 6, e.rest);
+    p[1] = and_or<0x00f000f0u>(w, e.first);
+    p[2] = and_or<0x03c003c0u>(w >> 2, e.rest);
+    p[3] = and_or<0x03c003c0u>(w >> 6, e.rest);
   }
   static constexpr uint32_t kOffset[4] = {0xce00ce00u, 0xd480d480u, 0xce00ce00u, 0xce00ce00u};  // -24, -72, ..
   static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

@@ -171,7 +171,7 @@ __device__ __forceinline__ uint4 decode_word(uint32_t w, uint32_t s2) {
   for (int b = 0; b < 4; ++b) {
     // byte b of w (its low nibble is k = 2b) and of w >> 4 (2b + 1)
     const uint32_t t = __byte_perm(w, v, b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12));
-    r[b] = Decode<T>::value(u4::and_or(t, 0x000f000fu, Decode<T>::kMagic), s2);
+    r[b] = Decode<T>::value(u4::and_or<0x000f000fu>(t, Decode<T>::kMagic), s2);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }

@@ -237,7 +237,7 @@ __device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* const (&
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int g = b * kPer + j;
-    if (g < groups) {
+    if (GROUP == 128 || g < groups) {
       const int at = g * (GROUP / 2);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -272,11 +272,12 @@ __device__ __forceinline__ void load_scales(Block4<T, GROUP, MT>& k, const T* co
   for (int j = 0; j < B::kPer; ++j) {
     const int g = b * B::kPer + j;
 #pragma unroll
-    for (int r = 0; r < B::kRows; ++r) k.s[r][j] = g < groups ? sc[r][g] : Act<T>::from_float(0.f);
+    for (int r = 0; r < B::kRows; ++r) k.s[r][j] = GROUP == 128 || g < groups ? __ldg(sc[r] + g) : Act<T>::from_float(0.f);
   }
 }
 
 // The activations of eight rows for the block: this lane's row, its words' k.
+// Lanes without a row read the last one's: their columns are not used.
 template <typename T, int GROUP>
 __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int groups) {
   using B = Block4<T, GROUP, 1>;
@@ -285,16 +286,15 @@ __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int 
 #pragma unroll
     for (int i = 0; i < B::kWords; ++i) {
       const int g = b * B::kPer + j;
-      v[j * B::kWords + i] = x != nullptr && g < groups
-                                 ? *reinterpret_cast<const uint4*>(x + (int64_t)g * GROUP + i * 8)
-                                 : make_uint4(0, 0, 0, 0);
+      v[j * B::kWords + i] = GROUP == 128 || g < groups ? __ldg(reinterpret_cast<const uint4*>(x + g * GROUP + i * 8))
+                                                        : make_uint4(0, 0, 0, 0);
     }
 }
 
 // acc += the block's products: MT tiles of sixteen weight rows by 8 NT tokens.
 template <typename T, int GROUP, int MT, int NT>
 __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Block4<T, GROUP, MT>& k,
-                                               const uint4 (&x)[NT][4]) {
+                                               const uint4 (&x)[NT][4], const u4::Exponents& ex) {
   using B = Block4<T, GROUP, MT>;
   constexpr uint32_t off_lo[4] = {Act<T>::kOffset[0], Act<T>::kOffset[0], Act<T>::kOffset[1], Act<T>::kOffset[1]};
   constexpr uint32_t off_hi[4] = {Act<T>::kOffset[2], Act<T>::kOffset[2], Act<T>::kOffset[3], Act<T>::kOffset[3]};
@@ -317,8 +317,8 @@ __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Bl
 #pragma unroll
       for (int i = 0; i < B::kWords; ++i) {
         uint32_t a0[4], a1[4];
-        Act<T>::decode(k.q[2 * m][j * B::kWords + i], a0);
-        Act<T>::decode(k.q[2 * m + 1][j * B::kWords + i], a1);
+        Act<T>::decode(k.q[2 * m][j * B::kWords + i], ex, a0);
+        Act<T>::decode(k.q[2 * m + 1][j * B::kWords + i], ex, a1);
         const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -423,7 +423,9 @@ __device__ __forceinline__ void group_barrier(int id, int threads) {
 
 // Blocks of 128 k whose words a warp has in flight.
 constexpr int kRowsDeep = 4;
-constexpr int kRowsSmem = kMvWarps * kRowsDeep * 2048;
+// Weight tiles of a warp and CTAs of an SM.
+__host__ __device__ constexpr int rows_tiles(int nt) { return 2; }
+__host__ __device__ constexpr int rows_ctas(int nt) { return 2; }
 
 // A place in a warp's run of work: the unit (an expert's strip), the chunk of
 // the expert's rows, the block of K.
@@ -433,18 +435,18 @@ struct RowsWork {
 };
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
-__global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams p) {
+__global__ void __launch_bounds__(kMvThreads, rows_ctas(NT)) int4_rows_kernel(const MvParams p) {
   pdl_begin();
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
   constexpr int kTokens = 8 * NT;
-  constexpr int kFeat = SWIGLU ? 16 : 32;  // output features of a strip
-  using B = Block4<T, GROUP, 2>;
-  constexpr int kBlockBytes = B::kBytes;
+  constexpr int MT = rows_tiles(NT);
+  constexpr int kFeat = (SWIGLU ? 8 : 16) * MT;  // output features of a strip
+  using B = Block4<T, GROUP, MT>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   extern __shared__ __align__(16) uint8_t s_words[];
   __shared__ RowLists s;
-  __shared__ float s_red[kMvWarps][32][kTokens + 1];
+  __shared__ float s_red[kMvWarps][16 * MT][kTokens + 1];
   list_rows(s, p);
 
   const int strips = (p.n_out + kFeat - 1) / kFeat;
@@ -473,8 +475,8 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
   auto weight_row = [&](int64_t unit, int r) -> int64_t {
     const int e = s.expert[unit / strips], strip = (int)(unit % strips);
     int row;
-    if (SWIGLU) row = min(strip * 16 + (r >> 1) * 8 + g, p.n_out - 1) + (r & 1) * p.n_out;
-    else row = min(strip * 32 + r * 8 + g, p.n_out - 1);
+    if (SWIGLU) row = min(strip * kFeat + (r >> 1) * 8 + g, p.n_out - 1) + (r & 1) * p.n_out;
+    else row = min(strip * kFeat + r * 8 + g, p.n_out - 1);
     return (int64_t)e * p.w_rows + row;
   };
   auto next = [&](RowsWork& w) -> bool {  // the next block; true: of another unit
@@ -489,62 +491,59 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_rows_kernel(const MvParams
 
   // neighbouring units on different CTAs: a small launch spreads over the SMs
   const RowsWork start{(int64_t)group * gridDim.x + blockIdx.x, 0, b0};
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_words) + warp * kRowsDeep * kBlockBytes + lane * 16;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_words) + warp * kRowsDeep * B::kBytes + lane * 16;
   RowsWork in = start;  // of the block copied next
-  const uint8_t* w[4] = {};
+  const uint8_t* w[2 * MT] = {};
   bool moved = true;
   auto copy_next = [&](int slot) {
     if (in.unit < units) {
       if (moved) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = p.w + weight_row(in.unit, r) * (p.K / 2) + t * 4 * kWords;
+        for (int r = 0; r < 2 * MT; ++r) w[r] = p.w + weight_row(in.unit, r) * (p.K / 2) + t * 4 * kWords;
       }
-      copy_words<GROUP>(ring + slot * kBlockBytes, w, in.b, kgroups);
+      copy_words<GROUP, 2 * MT>(ring + slot * B::kBytes, w, in.b, kgroups);
       moved = next(in);
     }
     copy_commit();
   };
 #pragma unroll 1
   for (int i = 0; i < kRowsDeep - 1; ++i) copy_next(i);
+  const u4::Exponents ex = Act<T>::exponents();
   int slot = 0;
   for (int64_t unit = start.unit; unit < units; unit += stride) {
     const int a = (int)(unit / strips), strip = (int)(unit % strips);
     const int first = s.first[a], cnt = s.rows[a];
-    const T* sc[4];
+    const T* sc[2 * MT];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sc[r] = static_cast<const T*>(p.scale) + weight_row(unit, r) * kgroups;
+    for (int r = 0; r < 2 * MT; ++r) sc[r] = static_cast<const T*>(p.scale) + weight_row(unit, r) * kgroups;
     for (int c0 = 0; c0 < cnt; c0 += kTokens) {
-      float acc[2][NT][4];
+      float acc[MT][NT][4];
       const T* xp[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[0][n][i] = acc[1][n][i] = 0.f;
-        const int i = c0 + n * 8 + g;
-        xp[n] = nullptr;
-        if (i < cnt) {
-          const int place = first + i;
-          const int row = p.ids ? s.list[place] / p.x_div : (p.row_map ? p.row_map[place] / p.x_div : place);
-          xp[n] = x + (int64_t)row * p.K + t * 8 * kWords;
-        }
+        for (int i = 0; i < 4 * MT; ++i) acc[i / 4][n][i % 4] = 0.f;
+        const int place = first + min(c0 + n * 8 + g, cnt - 1);
+        const int row = p.ids ? s.list[place] / p.x_div : (p.row_map ? p.row_map[place] / p.x_div : place);
+        xp[n] = x + (int64_t)row * p.K + t * 8 * kWords;
       }
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
         B k;
         uint4 xv[NT][4];
-        load_scales<T, GROUP, 2>(k, sc, b, kgroups);
+        load_scales<T, GROUP, MT>(k, sc, b, kgroups);
 #pragma unroll
         for (int n = 0; n < NT; ++n) load_acts<T, GROUP>(xv[n], xp[n], b, kgroups);
         // the slot freed by the last block takes the block kRowsDeep - 1 ahead
         copy_next(slot == 0 ? kRowsDeep - 1 : slot - 1);
         copy_wait<kRowsDeep - 1>();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) read_words(ring + slot * kBlockBytes + r * 512, k.q[r]);
-        multiply_block<T, GROUP, 2, NT>(acc, k, xv);
+        for (int r = 0; r < 2 * MT; ++r) read_words(ring + slot * B::kBytes + r * 512, k.q[r]);
+        multiply_block<T, GROUP, MT, NT>(acc, k, xv, ex);
         slot = slot + 1 == kRowsDeep ? 0 : slot + 1;
       }
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -674,6 +673,7 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
   for (int i = 0; i < kDownDeep - 1; ++i) copy_next(i);
   pdl_begin();  // h
 
+  const u4::Exponents ex = Act<T>::exponents();
   int slot = 0;
   int64_t at = lo;
   int tile = (int)(lo / blocks), b = (int)(lo % blocks);
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
     const T* sc[2] = {static_cast<const T*>(p.scale) + (base + r0) * kgroups,
                       static_cast<const T*>(p.scale) + (base + r1) * kgroups};
     const int rows = s_tile_rows[tile], first = s_tile_first[tile];
-    const T* xp = g < rows ? static_cast<const T*>(p.h) + (int64_t)s.list[first + g] * p.K + t * 8 * kWords : nullptr;
+    const T* xp = static_cast<const T*>(p.h) + (int64_t)s.list[first + min(g, rows - 1)] * p.K + t * 8 * kWords;
     const int end = (int)min((int64_t)blocks, b + (hi - at));
     float acc[1][1][4] = {};
     at += end - b;
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
       copy_wait<kDownDeep - 1>();
       read_words(ring + slot * B::kBytes, k.q[0]);
       read_words(ring + slot * B::kBytes + 512, k.q[1]);
-      multiply_block<T, GROUP, 1, 1>(acc, k, xv);
+      multiply_block<T, GROUP, 1, 1>(acc, k, xv, ex);
       slot = slot + 1 == kDownDeep ? 0 : slot + 1;
     }
     // column by column: two rows of a tile may belong to one token
@@ -798,11 +798,12 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
 int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
-  const int64_t units = ceil_div(p.n_out, SWIGLU ? 16 : 32) * std::min<int64_t>(p.E, rows);
-  const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), 2 * num_sms());
+  constexpr int kSmem = kMvWarps * kRowsDeep * Block4<T, GROUP, rows_tiles(NT)>::kBytes;
+  const int64_t units = ceil_div(p.n_out, (SWIGLU ? 8 : 16) * rows_tiles(NT)) * std::min<int64_t>(p.E, rows);
+  const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), rows_ctas(NT) * num_sms());
   auto kfn = int4_rows_kernel<T, GROUP, NT, SWIGLU>;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
-  MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)ctas), dim3(kMvThreads), kRowsSmem, st, p));
+  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)ctas), dim3(kMvThreads), kSmem, st, p));
   MOE_LAUNCH_CHECK("int4_rows_kernel");
   return MOE_OK;
 }
@@ -855,7 +856,7 @@ int launch_down_any(const DownParams& p, int dtype, int group, cudaStream_t st) 
 }
 
 // Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM).
-constexpr int64_t kRowsPerExpert = 16;
+constexpr int64_t kRowsPerExpert = 8;
 bool use_gemm(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
   const int opt = moe_get_option(MOE_OPT_INT4_GEMM);
   if (opt == 0 || rows == 0 || !int4_gemm_fits(rows, n_out, w_rows, E)) return false;
