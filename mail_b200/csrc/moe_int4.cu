@@ -349,9 +349,46 @@ struct RowLists {
   int active;  // experts listed
 };
 
+// Inclusive sum over the lanes of a warp.
+__device__ __forceinline__ int warp_inclusive(int v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += n;
+  }
+  return v;
+}
+
 __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
   __shared__ int64_t warp_sums[32];
   const int tid = threadIdx.x;
+  if (p.ids && p.slots <= 32) {
+    // a slot for each lane of one warp: experts in the order of their first slots
+    if (tid < 32) {
+      const int id = tid < p.slots ? p.ids[tid] : -1;
+      const bool live = id >= 0 && id < p.E;
+      const unsigned mates = __match_any_sync(0xffffffffu, live ? id : -1);
+      const unsigned below = (1u << tid) - 1;
+      const bool leads = live && (mates & below) == 0;
+      const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+      const int rows = leads ? __popc(mates) : 0;
+      const int incl = warp_inclusive(rows);
+      const int first = __shfl_sync(0xffffffffu, incl - rows, __ffs(mates) - 1);
+      if (leads) {
+        const int a = __popc(leaders & below);
+        s.expert[a] = id;
+        s.first[a] = first;
+        s.rows[a] = rows;
+      }
+      if (live) s.list[first + __popc(mates & below)] = tid;
+      if (tid == 31) {
+        s.total = incl;
+        s.active = __popc(leaders);
+      }
+    }
+    __syncthreads();
+    return;
+  }
   const int per = (p.E + kMvThreads - 1) / kMvThreads;
   const int lo = min(p.E, tid * per), hi = min(p.E, lo + per);
   if (p.ids) {
@@ -617,25 +654,28 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
   __shared__ RowLists s;
   __shared__ int s_tile_expert[kDownSlots], s_tile_first[kDownSlots], s_tile_rows[kDownSlots], s_tiles;
   __shared__ float s_sum[kMvWarps][kDownTokens][17];
-  __shared__ int64_t warp_sums[32];
 
   MvParams lists{};
   lists.ids = p.ids;
   lists.slots = p.slots;
   lists.E = p.E;
   list_rows(s, lists);
-  {
-    // tiles of up to eight rows of an expert (an expert for each thread at most)
-    const int rows = tid < s.active ? s.rows[tid] : 0;
-    const int64_t mine = (rows + 7) / 8;
-    const int64_t incl = block_inclusive_scan<int64_t>(mine, warp_sums);
-    for (int i = 0; i < (int)mine; ++i) {
-      const int at = (int)(incl - mine) + i;
-      s_tile_expert[at] = s.expert[tid];
-      s_tile_first[at] = s.first[tid] + 8 * i;
-      s_tile_rows[at] = min(8, rows - 8 * i);
+  if (warp == 0) {  // tiles of up to eight rows of an expert
+    int tiles = 0;
+    for (int a0 = 0; a0 < s.active; a0 += 32) {
+      const int a = a0 + lane;
+      const int rows = a < s.active ? s.rows[a] : 0;
+      const int mine = (rows + 7) / 8;
+      const int incl = warp_inclusive(mine);
+      for (int i = 0; i < mine; ++i) {
+        const int at = tiles + incl - mine + i;
+        s_tile_expert[at] = s.expert[a];
+        s_tile_first[at] = s.first[a] + 8 * i;
+        s_tile_rows[at] = min(8, rows - 8 * i);
+      }
+      tiles += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (tid == kMvThreads - 1) s_tiles = (int)incl;
+    if (lane == 0) s_tiles = tiles;
   }
   for (int i = lane; i < p.tokens * 17; i += 32) s_sum[warp][i / 17][i % 17] = 0.f;
   __syncthreads();
@@ -796,13 +836,26 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
   return MOE_OK;
 }
 
+// Lets KFN use `smem` bytes of dynamic shared memory, once for each device.
+template <auto KFN>
+int allow_smem(int smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  MOE_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return MOE_OK;
+  MOE_CUDA_TRY(cudaFuncSetAttribute(KFN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return MOE_OK;
+}
+
 template <typename T, int GROUP, int NT, bool SWIGLU>
 int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
   constexpr int kSmem = kMvWarps * kRowsDeep * Block4<T, GROUP, rows_tiles(NT)>::kBytes;
   const int64_t units = ceil_div(p.n_out, (SWIGLU ? 8 : 16) * rows_tiles(NT)) * std::min<int64_t>(p.E, rows);
   const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), rows_ctas(NT) * num_sms());
   auto kfn = int4_rows_kernel<T, GROUP, NT, SWIGLU>;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  MOE_TRY((allow_smem<int4_rows_kernel<T, GROUP, NT, SWIGLU>>(kSmem)));
   MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)ctas), dim3(kMvThreads), kSmem, st, p));
   MOE_LAUNCH_CHECK("int4_rows_kernel");
   return MOE_OK;
@@ -822,7 +875,7 @@ int launch_down(DownParams p, cudaStream_t st) {
   while (p.cluster < 8 && 2 * p.cluster * strips <= 2 * num_sms()) p.cluster *= 2;
   auto kfn = int4_down_kernel<T, GROUP>;
   const int smem = kMvWarps * kDownDeep * Block4<T, GROUP, 1>::kBytes;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  MOE_TRY((allow_smem<int4_down_kernel<T, GROUP>>(smem)));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3((unsigned)(strips * p.cluster));

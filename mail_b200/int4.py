@@ -127,16 +127,16 @@ def _check_weight(name: str, dtype: torch.dtype, w: torch.Tensor, scale: torch.T
     """Group size of a 4-bit weight [E, K / 2, N] with scales [E, N, K / g]."""
     if dtype not in _ACT:
         raise TypeError(f"{name}: 4-bit weights take bf16 or fp16 activations, not {dtype}")
-    if w.dim() != 3 or w.dtype != torch.uint8 or 2 * w.shape[1] != K:
+    ws, ss = w.shape, scale.shape
+    if len(ws) != 3 or w.dtype != torch.uint8 or 2 * ws[1] != K:
         raise ValueError(f"{name}: expected 4-bit weights uint8 [E, K / 2, N] with K = {K}, "
-                         f"got {w.dtype} {tuple(w.shape)}")
+                         f"got {w.dtype} {tuple(ws)}")
     if scale.dtype != dtype:
         raise TypeError(f"{name}: the scales must share the activations' type {dtype}, not {scale.dtype}")
-    if scale.dim() != 3 or tuple(scale.shape[:2]) != (w.shape[0], w.shape[2]) or scale.shape[2] == 0 \
-            or K % scale.shape[2]:
-        raise ValueError(f"{name}: scales {tuple(scale.shape)} do not fit weights {tuple(w.shape)} "
+    if len(ss) != 3 or ss[0] != ws[0] or ss[1] != ws[2] or ss[2] == 0 or K % ss[2]:
+        raise ValueError(f"{name}: scales {tuple(ss)} do not fit weights {tuple(ws)} "
                          "(expected [E, N, K / group_size])")
-    group_size = K // scale.shape[2]
+    group_size = K // ss[2]
     _check_group(name, K, group_size)
     return group_size
 
@@ -203,10 +203,11 @@ def fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
     E, H, inter, group, a, sa, b, sb = _layer_weights(x, w13, w2, w13_scale, w2_scale)
     dev = _one_device("fused_moe_mlp", x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale)
     x = x.contiguous()
-    wts = topk_weights.to(torch.float32).contiguous()
-    ids = topk_ids.to(torch.int32).contiguous()
+    wts = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.to(torch.float32)
+    ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
+    wts, ids = wts.contiguous(), ids.contiguous()
     T, k = ids.shape
-    y = torch.empty((T, H), dtype=x.dtype, device=dev)
+    y = x.new_empty((T, H))
     size = _lib.query("moe_fused_experts_int4_workspace_size", T, H, inter, E, k)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _launch(dev, "moe_fused_experts_int4", x.data_ptr(), _CODES[x.dtype], T, H, a.data_ptr(), sa.data_ptr(),
