@@ -391,6 +391,7 @@ __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
   }
   const int per = (p.E + kMvThreads - 1) / kMvThreads;
   const int lo = min(p.E, tid * per), hi = min(p.E, lo + per);
+  if (tid == 0) s.active = 0;
   if (p.ids) {
     for (int e = tid; e < p.E; e += kMvThreads) s.rows[e] = 0;
     __syncthreads();
@@ -422,18 +423,18 @@ __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
   int a = (int)((incl - mine) & 2047);
 #pragma unroll
   for (int i = 0; i < kMaxExperts / kMvThreads; ++i) {
-    if (cnt[i] > 0) {  // counts past the last row are cut off
-      s.expert[a] = lo + i;
-      s.first[a] = (int)min(run, limit);
-      s.rows[a] = (int)min((int64_t)cnt[i], max((int64_t)0, limit - run));
+    if (cnt[i] > 0) {
+      if (run < limit) {  // counts past the last row are cut off, and experts behind it not listed
+        s.expert[a] = lo + i;
+        s.first[a] = (int)run;
+        s.rows[a] = (int)min((int64_t)cnt[i], limit - run);
+        atomicMax(&s.active, a + 1);
+      }
       ++a;
       run += cnt[i];
     }
   }
-  if (tid == kMvThreads - 1) {
-    s.total = (int)min(incl >> 11, limit);
-    s.active = (int)(incl & 2047);
-  }
+  if (tid == kMvThreads - 1) s.total = (int)min(incl >> 11, limit);
   __syncthreads();
   if (p.ids) {
     // a slot's place: its expert's first, then one after the other

@@ -210,7 +210,8 @@ def test_grouped_matmul_random(dtype, K, N, group, sizes, kernel):
     assert_within(out, ref, (half_step(dtype) + 2 * K * 2.0 ** -24) * mag, dtype)
 
 
-@pytest.mark.parametrize("sizes", [[3, 0, 2], [0, 0, 0], [4, 4, 40], [-3, 5, 0], [12, 0, 0]])
+@pytest.mark.parametrize("sizes", [[3, 0, 2], [0, 0, 0], [4, 4, 40], [-3, 5, 0], [12, 0, 0], [12, 5, 7], [40, 0, 9],
+                                   [0, 13, 1]])
 def test_grouped_matmul_sizes_that_do_not_add_up(sizes, kernel):
     """Rows behind the last group are zero; counts past the rows are cut off;
     negative counts are empty groups."""
@@ -480,3 +481,23 @@ def test_refusals_on_the_device():
         mb.grouped_matmul_int4(x, w13, s13, torch.tensor([1, 2, 0, 3], device=DEV).cpu().pin_memory())
     with pytest.raises(TypeError, match="unsupported dtype"):
         mb.fused_expert_rows(x, w13, w2, ids[:, 0], scales=(s13, s2))
+
+
+def test_option_picks_the_kernel_and_its_default_stays():
+    lib = _lib.load()
+    assert lib.moe_get_option(_lib.OPT_INT4_GEMM) == 2
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, 3) == 1
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 4, 1), (32, 64, 1), (33, 64, 1), (32, 4, 4), (64, 128, 8), (130, 16, 8),
+                                   (40, 300, 3)])
+def test_layer_around_the_rules(T, E, k):
+    """Sizes on both sides of the rules that choose a kernel: 32 tokens, 256
+    and 1024 slots, eight rows an expert."""
+    H, I, group = 256, 128, 64
+    w13, s13, wide13 = weights(E, 2 * I, H, group, BF, 1)
+    w2, s2, wide2 = weights(E, H, I, group, BF, 2)
+    x = torch.randn((T, H), device=DEV, generator=gen(3)).to(BF)
+    wts, ids = routing(T, E, k, 4)
+    ref, bound = layer_ref(x, wide13, wide2, wts, ids, BF)
+    assert_within(mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2)), ref, bound, BF)
