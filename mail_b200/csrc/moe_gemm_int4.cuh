@@ -63,7 +63,9 @@ struct Int4Shape {
   static constexpr uint32_t kXBytes = kRows * ROW_BYTES;
   static constexpr int kThreads = 32 * (8 + 4 * kSets);
 };
-// Narrow tiles up to this many rows an expert on average.
+// Narrow tiles up to this many rows an expert on average. Narrow in us against
+// wide in us, 64 experts of 2048 x 1536: 32: 59 / 66, 48: 61 / 68, 64: 81 / 70;
+// 16 experts of 4096 x 4096: 32: 71 / 79, 48: 73 / 83, 64: 103 / 85.
 constexpr int64_t kInt4NarrowRows = 48;
 
 struct Int4Maps {

@@ -909,7 +909,10 @@ int launch_down_any(const DownParams& p, int dtype, int group, cudaStream_t st) 
   return launch_down<__half, 32>(p, st);
 }
 
-// Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM).
+// Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM). Rows in us against
+// tiles in us, by rows an expert, 128 experts of 2048 x 1536: 2: 60 / 87,
+// 4: 90 / 98, 8: 95 / 99, 12: 125 / 99; 8 experts of 4096 x 14336: 2: 72 / 105,
+// 8: 112 / 112, 12: 136 / 111.
 constexpr int64_t kRowsPerExpert = 8;
 bool use_gemm(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
   const int opt = moe_get_option(MOE_OPT_INT4_GEMM);
