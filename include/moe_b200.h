@@ -402,7 +402,12 @@ MOE_API int moe_fused_expert_rows(const void* x, int x_dtype, int64_t rows, int6
  * moe_fused_mlp_int4 / moe_fused_experts_int4: the layer in its pre-routed and
  * top-k forms (moe_fused_mlp, moe_fused_experts) with 4-bit weights. h is
  * rounded to x's type before the down projection. Tokens' rows are combined
- * in slot order, so results do not differ from run to run.
+ * in a fixed order, so results do not differ from run to run.
+ *
+ * Few rows an expert (MOE_OPT_INT4_GEMM) run without rounding a weight; the
+ * tensor-core tiles round each (q - 8) s once to x's type. A row of x that holds
+ * an infinity gives infinities or NaN in its own row of out only; magnitudes of
+ * 2^119 and more count as infinite (bf16).
  * -------------------------------------------------------------------------- */
 MOE_API int moe_quant_int4_groups(const void* src, int src_dtype, int64_t rows, int64_t cols, int group_size,
                                   uint8_t* dst, void* dst_scale, int scale_dtype, void* stream);

@@ -8,10 +8,16 @@
 // The 128 weight rows of a feature tile are the MMA's M operand and the
 // expert's rows (up to 256, evenly split over its tiles, rounded up to 16) its
 // N operand, so an expert with few rows costs few MMA columns. The tensor
-// cores take 16-bit operands: eight or twelve warps turn the 4-bit words into
+// cores take 16-bit operands: twelve or sixteen warps turn the 4-bit words into
 // (q - 8) s in shared memory while earlier blocks multiply. A weight is
 // rounded to the activations' type there, by at most half a step: scaling
 // after the product instead would read the accumulator once for every group.
+//
+// Measured: 8192 rows over eight experts of 4096 x 14336 759 us, 1268 TFLOP/s,
+// 0.77 of the measured burst (the part's power limit halves the margin in long
+// runs); 2048 rows over 64 experts of 7168 x 4096 396 us, 2.4 TB/s of weights,
+// bound by decoding and by the barriers between the roles (no decoding: 323 us,
+// no decoding, products or rows of x: 314 us).
 //
 // Roles (one CTA per SM, persistent), a warp each:
 //   issue      TMEM, MMAs into one of two accumulators
@@ -21,7 +27,7 @@
 //              themselves: the proxy fence after their stores would wait for
 //              every load in flight, a DRAM latency for each block.
 //   epilogue   four warps
-//   decode     two or three sets of four warps, a thread to a weight row
+//   decode     three or four sets of four warps, a thread to a weight row
 // With SWIGLU a tile's rows alternate between 16 gate rows and the 16 up rows
 // that go with them, so gate and up of a feature sit sixteen TMEM lanes apart
 // in one warp, and a shuffle for every two tokens brings them together.
