@@ -19,8 +19,8 @@ using u4::Act;
 // Quantising with group scales.
 //   s = T(absmax / 7)  (fp32 quotient, then the scales' type)
 //   q = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0
-// GROUP / 8 lanes share a group; a lane loads eight weights and stores their
-// four bytes. The rounding is that of the exact quotient, half to even. For
+// GROUP / 16 lanes share a group; a lane loads sixteen weights and stores their
+// eight bytes. The rounding is that of the exact quotient, half to even. For
 // 16-bit weights the correctly rounded fp32 quotient (a reciprocal for the
 // group, then one correction by the exact remainder) is enough: a quotient of
 // two such numbers that is not on a border is further from it than fp32's
@@ -33,57 +33,92 @@ using u4::Act;
 // takes 467 us, 5.2 TB/s of the 2.4 GB moved. A division for each weight bound
 // the quantiser by its instructions, about 30 a weight (806 us); now it has 8.
 
-// Eight weights as loaded, their largest magnitude (infinity or NaN if one is),
-// and as fp32. The bits of magnitudes are in the order of the numbers, with
-// infinity and NaN on top.
+// Sixteen weights as loaded, their largest magnitude (infinity or NaN if one
+// is), and eight of them as fp32. The bits of magnitudes are in the order of the
+// numbers, with infinity and NaN on top.
 template <typename T>
-struct Eight {
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+struct Sixteen {
+  uint4 raw[2];
+  __device__ __forceinline__ void load(const T* p) {
+    raw[0] = *reinterpret_cast<const uint4*>(p);
+    raw[1] = *reinterpret_cast<const uint4*>(p + 8);
+  }
+  __device__ __forceinline__ void zero() { raw[0] = raw[1] = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ float amax() const {
     constexpr uint32_t kAbs = 0x7fff7fffu;
-    const uint32_t m = __vmaxu2(__vmaxu2(raw.x & kAbs, raw.y & kAbs), __vmaxu2(raw.z & kAbs, raw.w & kAbs));
+    uint32_t m = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      m = __vmaxu2(m, __vmaxu2(__vmaxu2(raw[h].x & kAbs, raw[h].y & kAbs), __vmaxu2(raw[h].z & kAbs, raw[h].w & kAbs)));
     const uint16_t top = (uint16_t)max(m & 0xffffu, m >> 16);
     return Act<T>::to_float(*reinterpret_cast<const T*>(&top));
   }
-  __device__ __forceinline__ void floats(float (&v)[8]) const { rows::load8(reinterpret_cast<const T*>(&raw), v); }
+  __device__ __forceinline__ void floats(int half, float (&v)[8]) const {
+    rows::load8(reinterpret_cast<const T*>(&raw[half]), v);
+  }
 };
 template <>
-struct Eight<float> {
-  float f[8];
-  __device__ __forceinline__ void load(const float* p) { rows::load8(p, f); }
+struct Sixteen<float> {
+  float f[2][8];
+  __device__ __forceinline__ void load(const float* p) {
+    rows::load8(p, f[0]);
+    rows::load8(p + 8, f[1]);
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    for (int j = 0; j < 16; ++j) f[j / 8][j % 8] = 0.f;
   }
   __device__ __forceinline__ float amax() const {
     int bits = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_int(f[j]) & 0x7fffffff);
+    for (int j = 0; j < 16; ++j) bits = max(bits, __float_as_int(f[j / 8][j % 8]) & 0x7fffffff);
     return __int_as_float(bits);
   }
-  __device__ __forceinline__ void floats(float (&v)[8]) const {
+  __device__ __forceinline__ void floats(int half, float (&v)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = f[j];
+    for (int j = 0; j < 8; ++j) v[j] = f[half][j];
   }
 };
 
+// The eight steps of one word, s > 0 and its reciprocal given.
+template <bool EXACT_QUOTIENT>
+__device__ __forceinline__ uint32_t quant_word(const float (&v)[8], float s, float inv) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float t;  // kRound + the step
+    if constexpr (EXACT_QUOTIENT) {
+      const float quot = v[j] * inv;
+      t = fmaf(fmaf(-quot, s, v[j]), inv, quot) + kRound;
+    } else {
+      t = fmaf(v[j], inv, kRound);
+      const float rest = fmaf(kRound - t, s, v[j]);
+      const float past = fmaf(2.f, fabsf(rest), -s);  // > 0: beyond half a step, 0: on the border
+      if (past > 0.f || (past == 0.f && (__float_as_int(t) & 1))) t += rest > 0.f ? 1.f : -1.f;
+    }
+    word += (uint32_t)__float_as_int(t) << (4 * j);
+  }
+  // the bits of kRound out of every place, 8 into it: a step is in -8 .. 7
+  constexpr uint32_t kBits = 0x4b400000u;
+  constexpr uint32_t kOut = kBits * 0x11111111u;
+  return word - kOut + 0x88888888u;
+}
+
 template <typename Tw, typename Ts, int GROUP>
-__global__ void __launch_bounds__(256) quant_groups_kernel(const Tw* __restrict__ src, int64_t n8,
-                                                           uint32_t* __restrict__ dst, Ts* __restrict__ scale) {
+__global__ void __launch_bounds__(256) quant_groups_kernel(const Tw* __restrict__ src, int64_t n16,
+                                                           uint2* __restrict__ dst, Ts* __restrict__ scale) {
   pdl_begin();
-  constexpr int kLanes = GROUP / 8;
-  constexpr int kVec = sizeof(Tw) == 2 ? 4 : 2;            // vectors of eight in flight
-  constexpr float kRound = 12582912.f;                     // 1.5 * 2^23: adding it rounds to a whole number
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;  // a multiple of kLanes: a group's lanes stay together
-  const int64_t last = (n8 + 31) / 32 * 32;                // whole warps take part in the shuffles
+  constexpr int kLanes = GROUP / 16;
+  constexpr int kVec = sizeof(Tw) == 2 ? 2 : 1;             // vectors of sixteen in flight
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;   // a multiple of kLanes: a group's lanes stay together
+  const int64_t last = (n16 + 31) / 32 * 32;                // whole warps take part in the shuffles
   for (int64_t base = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; base < last; base += kVec * stride) {
-    Eight<Tw> in[kVec];
+    Sixteen<Tw> in[kVec];
 #pragma unroll
     for (int u = 0; u < kVec; ++u) {
       const int64_t i = base + u * stride;
-      if (i < n8) in[u].load(src + i * 8);
+      if (i < n16) in[u].load(src + i * 16);
       else in[u].zero();
     }
 #pragma unroll
@@ -95,39 +130,26 @@ __global__ void __launch_bounds__(256) quant_groups_kernel(const Tw* __restrict_
       for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
       Ts st = Act<Ts>::from_float(__fdiv_rn(__int_as_float(bits), 7.0f));
       float s = Act<Ts>::to_float(st);
-      uint32_t word = 0x88888888u;
+      uint2 words = make_uint2(0x88888888u, 0x88888888u);
       if (!isfinite(s)) {
         st = Act<Ts>::from_float(NAN);
       } else if (s > 0.f) {
-        float v[8];
-        in[u].floats(v);
+        float v[2][8];
+        in[u].floats(0, v[0]);
+        in[u].floats(1, v[1]);
         if (s < 6.2e-5f) {
           // a scale that may be subnormal: it can be well below absmax / 7, so
           // the steps are clamped, and its reciprocal may overflow
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -8.f * s), 7.f * s) * 0x1p64f;
+          for (int j = 0; j < 16; ++j) v[j / 8][j % 8] = fminf(fmaxf(v[j / 8][j % 8], -8.f * s), 7.f * s) * 0x1p64f;
           s *= 0x1p64f;
         }
         const float inv = __frcp_rn(s);
-        word = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float t;  // kRound + the step
-          if constexpr (sizeof(Tw) == 2) {
-            const float quot = v[j] * inv;
-            t = fmaf(fmaf(-quot, s, v[j]), inv, quot) + kRound;
-          } else {
-            t = fmaf(v[j], inv, kRound);
-            const float rest = fmaf(kRound - t, s, v[j]);
-            const float past = fmaf(2.f, fabsf(rest), -s);  // > 0: beyond half a step, 0: on the border
-            if (past > 0.f || (past == 0.f && (__float_as_int(t) & 1))) t += rest > 0.f ? 1.f : -1.f;
-          }
-          word += (uint32_t)(__float_as_int(t) - __float_as_int(kRound)) << (4 * j);
-        }
-        word += 0x88888888u;  // eight carries at most: a step is in -8 .. 7
+        words.x = quant_word<sizeof(Tw) == 2>(v[0], s, inv);
+        words.y = quant_word<sizeof(Tw) == 2>(v[1], s, inv);
       }
-      if (i < n8) {
-        dst[i] = word;
+      if (i < n16) {
+        dst[i] = words;
         if (i % kLanes == 0) scale[i / kLanes] = st;
       }
     }
@@ -815,10 +837,10 @@ unsigned flat_grid(int64_t threads) {
 }
 
 template <typename Tw, typename Ts>
-int launch_quant(const void* src, int64_t n8, int group, void* dst, void* scale, cudaStream_t st) {
+int launch_quant(const void* src, int64_t n16, int group, void* dst, void* scale, cudaStream_t st) {
 #define MOE_QUANT(G)                                                                                      \
-  MOE_CUDA_TRY(launch_kernel(quant_groups_kernel<Tw, Ts, G>, dim3(flat_grid(n8)), dim3(256), 0, st,        \
-                             static_cast<const Tw*>(src), n8, static_cast<uint32_t*>(dst), static_cast<Ts*>(scale)))
+  MOE_CUDA_TRY(launch_kernel(quant_groups_kernel<Tw, Ts, G>, dim3(flat_grid(n16)), dim3(256), 0, st,       \
+                             static_cast<const Tw*>(src), n16, static_cast<uint2*>(dst), static_cast<Ts*>(scale)))
   if (group == 128) MOE_QUANT(128);
   else if (group == 64) MOE_QUANT(64);
   else MOE_QUANT(32);
@@ -1004,18 +1026,18 @@ extern "C" int moe_quant_int4_groups(const void* src, int src_dtype, int64_t row
                 (long long)cols, group_size);
   if (rows == 0) return MOE_OK;
   MOE_CHECK_ARG(src && dst && dst_scale, "moe_quant_int4_groups: NULL pointer");
-  MOE_CHECK_ARG((uintptr_t)src % 16 == 0 && (uintptr_t)dst % 4 == 0,
-                "moe_quant_int4_groups: source must be 16-byte and output 4-byte aligned");
-  const int64_t n8 = rows * cols / 8;
+  MOE_CHECK_ARG((uintptr_t)src % 16 == 0 && (uintptr_t)dst % 8 == 0,
+                "moe_quant_int4_groups: source must be 16-byte and output 8-byte aligned");
+  const int64_t n16 = rows * cols / 16;
   cudaStream_t st = as_stream(stream);
   if (scale_dtype == MOE_BF16) {
-    if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
-    if (src_dtype == MOE_F16) return launch_quant<__half, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
-    return launch_quant<float, __nv_bfloat16>(src, n8, group_size, dst, dst_scale, st);
+    if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __nv_bfloat16>(src, n16, group_size, dst, dst_scale, st);
+    if (src_dtype == MOE_F16) return launch_quant<__half, __nv_bfloat16>(src, n16, group_size, dst, dst_scale, st);
+    return launch_quant<float, __nv_bfloat16>(src, n16, group_size, dst, dst_scale, st);
   }
-  if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __half>(src, n8, group_size, dst, dst_scale, st);
-  if (src_dtype == MOE_F16) return launch_quant<__half, __half>(src, n8, group_size, dst, dst_scale, st);
-  return launch_quant<float, __half>(src, n8, group_size, dst, dst_scale, st);
+  if (src_dtype == MOE_BF16) return launch_quant<__nv_bfloat16, __half>(src, n16, group_size, dst, dst_scale, st);
+  if (src_dtype == MOE_F16) return launch_quant<__half, __half>(src, n16, group_size, dst, dst_scale, st);
+  return launch_quant<float, __half>(src, n16, group_size, dst, dst_scale, st);
 }
 
 extern "C" int moe_dequant_int4_groups(const uint8_t* src, const void* scale, int scale_dtype, int64_t rows,
