@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
   const int E = p.E;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.raw; ++i) {
-      ptx::mbar_init(&sm.raw_full[i], 2);   // words, scales
+      ptx::mbar_init(&sm.raw_full[i], 1 + 32);  // words, the lanes that store the scales
       ptx::mbar_init(&sm.raw_empty[i], 8);  // the warps of two sets, one for each half
     }
     for (int i = 0; i < kStages; ++i) {
@@ -594,8 +594,7 @@ __global__ void __launch_bounds__(Int4Shape<NARROW>::kThreads, 1)
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int j = 0; j < NS; ++j) dst[(q * 32 + lane) * NS + j] = v[i][q][j];
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&sm.raw_full[slot]);
+        ptx::mbar_arrive(&sm.raw_full[slot]);  // every lane, for its own stores
         load(v[i]);
         if (++slot == p.raw) {
           slot = 0;
