@@ -490,7 +490,7 @@ def test_option_picks_the_kernel_and_its_default_stays():
 
 
 @pytest.mark.parametrize("T,E,k", [(1, 4, 1), (32, 64, 1), (33, 64, 1), (32, 4, 4), (64, 128, 8), (130, 16, 8),
-                                   (40, 300, 3)])
+                                   (40, 300, 3), (2500, 8, 8)])
 def test_layer_around_the_rules(T, E, k):
     """Sizes on both sides of the rules that choose a kernel: 32 tokens, 256
     and 1024 slots, eight rows an expert."""
@@ -501,3 +501,41 @@ def test_layer_around_the_rules(T, E, k):
     wts, ids = routing(T, E, k, 4)
     ref, bound = layer_ref(x, wide13, wide2, wts, ids, BF)
     assert_within(mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2)), ref, bound, BF)
+
+
+def test_empty_batches():
+    w13, s13, _ = weights(4, 256, 128, 64, BF, 1)
+    w2, s2, _ = weights(4, 128, 128, 64, BF, 2)
+    x = torch.empty((0, 128), dtype=BF, device=DEV)
+    ids = torch.empty((0, 2), dtype=torch.int32, device=DEV)
+    y = mb.fused_moe_mlp(x, w13, w2, torch.empty((0, 2), device=DEV), ids, scales=(s13, s2))
+    assert y.shape == (0, 128) and y.dtype == BF
+    assert mb.fused_moe_mlp(x, w13, w2, torch.zeros(4, dtype=torch.int64, device=DEV),
+                            scales=(s13, s2)).shape == (0, 128)
+    with pytest.raises(ValueError, match="need scales"):
+        mb.fused_moe_mlp(x, w13, w2, torch.zeros(4, dtype=torch.int64, device=DEV))
+
+
+def test_layer_takes_other_routing_types_and_strides():
+    """int64 ids, bf16 weights, strided activations, ids and weights: what the
+    layer takes with other weights, it takes here."""
+    E, H, I, k, T = 8, 256, 128, 2, 40
+    w13, s13, wide13 = weights(E, 2 * I, H, 64, BF, 1)
+    w2, s2, wide2 = weights(E, H, I, 64, BF, 2)
+    x = torch.randn((2 * T, 2 * H), device=DEV, generator=gen(3)).to(BF)[::2, H:]
+    wts, ids = routing(T, E, k, 4)
+    want = mb.fused_moe_mlp(x.contiguous(), w13, w2, wts, ids, scales=(s13, s2))
+    many = torch.stack((ids.long(), ids.long() + 1), dim=2)[:, :, 0]
+    assert torch.equal(mb.fused_moe_mlp(x, w13, w2, wts.t().contiguous().t(), many, scales=(s13, s2)), want)
+    rounded = mb.fused_moe_mlp(x, w13, w2, wts.to(BF).float(), ids, scales=(s13, s2))
+    assert torch.equal(mb.fused_moe_mlp(x, w13, w2, wts.to(BF), ids, scales=(s13, s2)), rounded)
+    grown = torch.cat((s13, s13), dim=2)[:, :, :s13.shape[2]]
+    assert not grown.is_contiguous()
+    assert torch.equal(mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(grown, s2)), want)
+
+
+def test_misaligned_activations_are_refused():
+    w, s, _ = weights(2, 32, 128, 64, BF, 1)
+    x = torch.zeros(4 * 128 + 1, dtype=BF, device=DEV)[1:].view(4, 128)
+    with pytest.raises(mb.MoeError, match="aligned"):
+        mb.grouped_matmul_int4(x, w, s, torch.tensor([2, 2], device=DEV))
