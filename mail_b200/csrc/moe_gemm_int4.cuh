@@ -13,9 +13,8 @@
 // rounded to the activations' type there, by at most half a step: scaling
 // after the product instead would read the accumulator once for every group.
 //
-// Measured: 8192 rows over eight experts of 4096 x 14336 759 us, 1268 TFLOP/s,
-// 0.77 of the measured burst (the part's power limit halves the margin in long
-// runs); 2048 rows over 64 experts of 7168 x 4096 396 us, 2.4 TB/s of weights,
+// Measured: 8192 rows over eight experts of 4096 x 14336 738 us, 1304 TFLOP/s,
+// 0.79 of the measured burst (878 us back to back, under the power limit); 2048 rows over 64 experts of 7168 x 4096 396 us, 2.4 TB/s of weights,
 // bound by decoding and by the barriers between the roles (no decoding: 323 us,
 // no decoding, products or rows of x: 314 us).
 //
@@ -71,7 +70,9 @@ struct Int4Shape {
 };
 // Narrow tiles up to this many rows an expert on average. Narrow in us against
 // wide in us, 64 experts of 2048 x 1536: 32: 59 / 66, 48: 61 / 68, 64: 81 / 70;
-// 16 experts of 4096 x 4096: 32: 71 / 79, 48: 73 / 83, 64: 103 / 85.
+// 16 experts of 4096 x 4096: 32: 71 / 79, 48: 73 / 83, 64: 103 / 85. Narrow as
+// well where all of them run at once (777 rows, 5 experts of 1056 x 1001: 18.7 /
+// 20.6; not so, 600 rows, 2 experts of 7168 x 2048: 62 / 47).
 constexpr int64_t kInt4NarrowRows = 48;
 
 struct Int4Maps {
@@ -711,7 +712,8 @@ int launch_int4_gemm(const Int4Maps& maps, Int4Params p, int64_t rows_hit, cudaS
 
 template <typename T, int GROUP>
 int launch_int4_shape(bool swiglu, const Int4Maps& maps, const Int4Params& p, int64_t hit, cudaStream_t st) {
-  if (p.total_rows <= kInt4NarrowRows * hit)
+  const int64_t narrow_items = (ceil_div(p.total_rows, Int4Shape<true>::kRows) + hit) * p.nf;
+  if (p.total_rows <= kInt4NarrowRows * hit || narrow_items <= num_sms())
     return swiglu ? launch_int4_gemm<T, GROUP, true, true>(maps, p, hit, st)
                   : launch_int4_gemm<T, GROUP, false, true>(maps, p, hit, st);
   return swiglu ? launch_int4_gemm<T, GROUP, true, false>(maps, p, hit, st)

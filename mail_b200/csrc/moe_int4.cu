@@ -30,8 +30,9 @@ using u4::Act;
 // gets a NaN scale and q = 8, so what it stands for shows as NaN.
 //
 // Both directions stream: 32768 x 14336 bf16 in groups of 32, there and back,
-// takes 467 us, 5.2 TB/s of the 2.4 GB moved. A division for each weight bound
-// the quantiser by its instructions, about 30 a weight (806 us); now it has 8.
+// takes 414 us, 5.8 TB/s of the 2.4 GB moved (467 with eight weights a lane).
+// A division for each weight bound the quantiser by its instructions, about 30
+// a weight (806 us).
 
 // Sixteen weights as loaded, their largest magnitude (infinity or NaN if one
 // is), and eight of them as fp32. The bits of magnitudes are in the order of the
