@@ -14,9 +14,10 @@
 // after the product instead would read the accumulator once for every group.
 //
 // Measured: 8192 rows over eight experts of 4096 x 14336 738 us, 1304 TFLOP/s,
-// 0.79 of the measured burst (878 us back to back, under the power limit); 2048 rows over 64 experts of 7168 x 4096 396 us, 2.4 TB/s of weights,
-// bound by decoding and by the barriers between the roles (no decoding: 323 us,
-// no decoding, products or rows of x: 314 us).
+// 0.79 of the measured burst (878 us back to back, under the power limit);
+// 2048 rows over 64 experts of 7168 x 4096 396 us, 2.4 TB/s of weights, bound by
+// decoding and by the barriers between the roles (no decoding: 323 us, no
+// decoding, products or rows of x: 314 us).
 //
 // Roles (one CTA per SM, persistent), a warp each:
 //   issue      TMEM, MMAs into one of two accumulators
