@@ -221,6 +221,7 @@ constexpr int kMvThreads = 256;
 constexpr int kMvWarps = kMvThreads / 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 1024;  // routed slots of the form that reads top-k ids
+constexpr int kDownSlots = 256;  // and of the fused down projection
 
 struct MvParams {
   const void* x;         // [.., K]
@@ -367,7 +368,9 @@ __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Bl
 
 // The experts that have rows, in order: expert, first place in the list of
 // rows, number of rows. Rows in counts form are the places themselves; in ids
-// form s.list holds the slots expert by expert (in no particular order).
+// form s.list holds the slots expert by expert: with IN_ORDER those of an expert
+// in order, the same for every CTA and in every run; else as the warps arrive,
+// which is enough where a row's values do not depend on its place.
 struct RowLists {
   int expert[kMaxExperts], first[kMaxExperts], rows[kMaxExperts];
   int list[kMaxSlots];
@@ -385,9 +388,13 @@ __device__ __forceinline__ int warp_inclusive(int v) {
   return v;
 }
 
-__device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
+// seen [kMaxExperts], IN_ORDER only: shared memory that is free until the
+// return. It holds, for each expert, how many of its slots each of the eight
+// warps has, a byte for a warp.
+template <bool IN_ORDER>
+__device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p, uint2* seen) {
   __shared__ int64_t warp_sums[32];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (p.ids && p.slots <= 32) {
     // a slot for each lane of one warp: experts in the order of their first slots
     if (tid < 32) {
@@ -418,12 +425,29 @@ __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
   const int per = (p.E + kMvThreads - 1) / kMvThreads;
   const int lo = min(p.E, tid * per), hi = min(p.E, lo + per);
   if (tid == 0) s.active = 0;
+  // IN_ORDER: thread t takes slot t. Its place among its expert's slots is the
+  // number of them before it: in its warp here, and in the warps below. (In
+  // order for up to 1024 slots, four a thread: 218 us for the layer of 128 experts
+  // at 128 tokens, 211 this way.)
+  static_assert(kDownSlots <= kMvThreads && kMvWarps == 8, "a slot a thread, a byte of seen for each warp");
+  int id = -1, before = 0;
   if (p.ids) {
-    for (int e = tid; e < p.E; e += kMvThreads) s.rows[e] = 0;
+    for (int e = tid; e < p.E; e += kMvThreads) {
+      if constexpr (IN_ORDER) seen[e] = make_uint2(0, 0);
+      else s.rows[e] = 0;
+    }
     __syncthreads();
-    for (int i = tid; i < p.slots; i += kMvThreads) {
-      const int e = p.ids[i];
-      if (e >= 0 && e < p.E) atomicAdd(&s.rows[e], 1);
+    if constexpr (IN_ORDER) {
+      if (tid < p.slots) id = p.ids[tid];
+      if (id < 0 || id >= p.E) id = -1;
+      const unsigned mates = __match_any_sync(0xffffffffu, id);
+      before = __popc(mates & ((1u << lane) - 1));
+      if (id >= 0 && before == 0) reinterpret_cast<uint8_t*>(&seen[id])[warp] = (uint8_t)__popc(mates);
+    } else {
+      for (int i = tid; i < p.slots; i += kMvThreads) {
+        const int e = p.ids[i];
+        if (e >= 0 && e < p.E) atomicAdd(&s.rows[e], 1);
+      }
     }
     __syncthreads();
   }
@@ -434,7 +458,12 @@ __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
     cnt[i] = 0;
     if (lo + i < hi) {
       if (p.ids) {
-        cnt[i] = s.rows[lo + i];
+        if constexpr (IN_ORDER) {
+          const uint2 v = seen[lo + i];
+          cnt[i] = (int)__dp4a(v.x, 0x01010101u, __dp4a(v.y, 0x01010101u, 0u));
+        } else {
+          cnt[i] = s.rows[lo + i];
+        }
       } else {
         const int64_t c = p.counts_is64 ? static_cast<const int64_t*>(p.counts)[lo + i]
                                         : (int64_t) static_cast<const int32_t*>(p.counts)[lo + i];
@@ -463,20 +492,31 @@ __device__ __forceinline__ void list_rows(RowLists& s, const MvParams& p) {
   if (tid == kMvThreads - 1) s.total = (int)min(incl >> 11, limit);
   __syncthreads();
   if (p.ids) {
-    // a slot's place: its expert's first, then one after the other
-    for (int i = tid; i < p.slots; i += kMvThreads) {
-      const int e = p.ids[i];
-      if (e < 0 || e >= p.E) continue;
+    auto listed = [&](int e) {  // place of expert e among those listed
       int l = 0, h = s.active - 1;
       while (l < h) {
         const int m = (l + h) >> 1;
         if (s.expert[m] < e) l = m + 1;
         else h = m;
       }
-      s.list[atomicAdd(&s.first[l], 1)] = i;
+      return l;
+    };
+    if constexpr (IN_ORDER) {
+      if (id >= 0) {
+        const uint2 v = seen[id];  // the bytes of the warps below are added
+        const uint32_t lo4 = warp < 4 ? (1u << (8 * warp)) - 1 : 0xffffffffu;
+        const uint32_t hi4 = warp < 4 ? 0u : (1u << (8 * (warp - 4))) - 1;
+        before += (int)__dp4a(v.x & lo4, 0x01010101u, __dp4a(v.y & hi4, 0x01010101u, 0u));
+        s.list[s.first[listed(id)] + before] = tid;
+      }
+    } else {  // its expert's first, then one after the other
+      for (int i = tid; i < p.slots; i += kMvThreads) {
+        const int e = p.ids[i];
+        if (e >= 0 && e < p.E) s.list[atomicAdd(&s.first[listed(e)], 1)] = i;
+      }
+      __syncthreads();
+      for (int i = tid; i < s.active; i += kMvThreads) s.first[i] -= s.rows[i];
     }
-    __syncthreads();
-    for (int i = tid; i < s.active; i += kMvThreads) s.first[i] -= s.rows[i];
     __syncthreads();
   }
 }
@@ -511,7 +551,7 @@ __global__ void __launch_bounds__(kMvThreads, rows_ctas(NT)) int4_rows_kernel(co
   extern __shared__ __align__(16) uint8_t s_words[];
   __shared__ RowLists s;
   __shared__ float s_red[kMvWarps][16 * MT][kTokens + 1];
-  list_rows(s, p);
+  list_rows<false>(s, p, nullptr);
 
   const int strips = (p.n_out + kFeat - 1) / kFeat;
   const int blocks = (int)((p.K + 127) / 128);
@@ -654,11 +694,11 @@ __global__ void __launch_bounds__(kMvThreads, rows_ctas(NT)) int4_rows_kernel(co
 // their tiles, times the routing weights, to sums of their own for each token.
 // Those are added over the warps of a CTA, then over the CTAs of the cluster
 // through distributed shared memory, always in the same order, and rounded
-// once: no atomics, no buffer of rows, and no third launch. The lists and the
+// once: no buffer of rows and no third launch. All CTAs of a cluster have to cut
+// the same tiles from the lists, so these are in order (list_rows). The lists and the
 // first words do not depend on h, so they are read before the wait for the
 // gate_up launch (which itself has waited for whatever wrote ids and weights).
 constexpr int kDownTokens = 32;
-constexpr int kDownSlots = 256;
 constexpr int kDownDeep = 6;
 
 struct DownParams {
@@ -680,13 +720,14 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
   extern __shared__ __align__(16) uint8_t s_words[];
   __shared__ RowLists s;
   __shared__ int s_tile_expert[kDownSlots], s_tile_first[kDownSlots], s_tile_rows[kDownSlots], s_tiles;
-  __shared__ float s_sum[kMvWarps][kDownTokens][17];
+  __shared__ __align__(16) float s_sum[kMvWarps][kDownTokens][17];
+  static_assert(sizeof(s_sum) >= kMaxExperts * sizeof(uint2), "list_rows needs it for a while");
 
   MvParams lists{};
   lists.ids = p.ids;
   lists.slots = p.slots;
   lists.E = p.E;
-  list_rows(s, lists);
+  list_rows<true>(s, lists, reinterpret_cast<uint2*>(s_sum));
   if (warp == 0) {  // tiles of up to eight rows of an expert
     int tiles = 0;
     for (int a0 = 0; a0 < s.active; a0 += 32) {

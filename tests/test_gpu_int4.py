@@ -539,3 +539,33 @@ def test_misaligned_activations_are_refused():
     x = torch.zeros(4 * 128 + 1, dtype=BF, device=DEV)[1:].view(4, 128)
     with pytest.raises(mb.MoeError, match="aligned"):
         mb.grouped_matmul_int4(x, w, s, torch.tensor([2, 2], device=DEV))
+
+
+@pytest.mark.parametrize("repeats", [False, True])
+@pytest.mark.parametrize("T,E,k,H", [(32, 32, 8, 256), (32, 32, 8, 1024), (32, 32, 8, 2048), (32, 32, 8, 4096),
+                                     (20, 8, 3, 1024), (32, 128, 8, 2048), (100, 128, 8, 256)])
+def test_decode_batch_with_crowded_experts(T, E, k, H, repeats):
+    """33 slots and more with several tiles of rows for one expert: every CTA has
+    to cut the same tiles from the routing, call after call. (The hidden sizes
+    give clusters of eight, four or two CTAs a strip, and one alone.)"""
+    I, group = 768, 64
+    w13, s13, wide13 = weights(E, 2 * I, H, group, BF, 1)
+    w2, s2, wide2 = weights(E, H, I, group, BF, 2)
+    x = torch.randn((T, H), device=DEV, generator=gen(3)).to(BF)
+    score = torch.rand((T, E), device=DEV, generator=gen(4))
+    for e, rows in enumerate((32, 17, 16, 9)[:k - 1]):  # tokens that name expert e
+        score[:, e] += 10 * (torch.randperm(T, device=DEV, generator=gen(5 + e)) < rows) - 5
+    top, ids = torch.topk(score, k, dim=1)
+    wts, ids = torch.softmax(top % 1, dim=1).float(), ids.to(torch.int32)
+    if repeats:  # the first two slots of every other token name one expert, some slots none
+        ids[::2, 1] = ids[::2, 0]
+        ids[1::4, -1] = -1
+    assert 32 < T * k <= 8 * E
+    ref, bound = layer_ref(x, wide13, wide2, wts, ids, BF)
+    first = mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2))
+    assert_within(first, ref, bound, BF)
+    differ = torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(400):
+        differ += (mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2)) != first).any()
+    assert int(differ) == 0, f"{int(differ)} of 400 calls differ from the first"
+    assert mb.device_error() == 0
