@@ -46,19 +46,22 @@ struct Act;
 
 template <>
 struct Act<__nv_bfloat16> {
-  // M + q of word w: pairs (k0, k4) with M = 128, from the lowest four mantissa
-  // bits as they stand; (k1, k5), (k2, k6), (k3, k7) with M = 16, shifted to
-  // the highest four. Left as it is, M costs no instruction for each weight;
-  // kOffset, -(M + 8), multiplied by the same
-  // activations, takes it out of the sums.
-  static __device__ __forceinline__ Exponents exponents() { return held_exponents<0x43004300u, 0x41804180u>(); }
+  // (M + q) / kUnit of word w: pairs (k0, k4) with M = 128, from the lowest four
+  // mantissa bits as they stand; (k1, k5), (k2, k6), (k3, k7) with M = 16, shifted
+  // to the highest four. Left as it is, M costs no instruction for each weight;
+  // kOffset, -(M + 8) / kUnit, multiplied by the same activations, takes it out
+  // of the sums. The largest M + q of a group of 128 add up to less than 2^13, so
+  // in units of 2^13 no group's sum overflows, whatever the activations are; at
+  // the other end the unit costs sums 2^-136, an eighth of bf16's smallest step.
+  static constexpr float kUnit = 8192.f;
+  static __device__ __forceinline__ Exponents exponents() { return held_exponents<0x3c803c80u, 0x3b003b00u>(); }
   static __device__ __forceinline__ void decode(uint32_t w, const Exponents& e, uint32_t (&p)[4]) {
     p[0] = and_or<0x000f000fu>(w, e.first);
     p[1] = and_or<0x00780078u>(w >> 1, e.rest);
     p[2] = and_or<0x00780078u>(w >> 5, e.rest);
     p[3] = and_or<0x00780078u>(w >> 9, e.rest);
   }
-  static constexpr uint32_t kOffset[4] = {0xc308c308u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};  // -136, -24, ..
+  static constexpr uint32_t kOffset[4] = {0xbc88bc88u, 0xbb40bb40u, 0xbb40bb40u, 0xbb40bb40u};  // -136, -24, ..
   static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
   // d = a b + c, d = a b, d += a b
@@ -84,7 +87,9 @@ struct Act<__nv_bfloat16> {
 template <>
 struct Act<__half> {
   // M + q: ten mantissa bits take (k1, k5) as it stands, with M = 64; the other
-  // pairs shifted to the highest four, with M = 16
+  // pairs shifted to the highest four, with M = 16. (Sums of fp16 activations
+  // are far from fp32's limits.)
+  static constexpr float kUnit = 1.f;
   static __device__ __forceinline__ Exponents exponents() { return held_exponents<0x54005400u, 0x4c004c00u>(); }
   static __device__ __forceinline__ void decode(uint32_t w, const Exponents& e, uint32_t (&p)[4]) {
     p[0] = and_or<0x03c003c0u>(w << 6, e.rest);

@@ -318,7 +318,8 @@ __device__ __forceinline__ void load_acts(uint4 (&v)[4], const T* x, int b, int 
     }
 }
 
-// acc += the block's products: MT tiles of sixteen weight rows by 8 NT tokens.
+// acc += the block's products, in units of kUnit: MT tiles of sixteen weight rows
+// by 8 NT tokens.
 template <typename T, int GROUP, int MT, int NT>
 __device__ __forceinline__ void multiply_block(float (&acc)[MT][NT][4], const Block4<T, GROUP, MT>& k,
                                                const uint4 (&x)[NT][4], const u4::Exponents& ex) {
@@ -665,7 +666,8 @@ __global__ void __launch_bounds__(kMvThreads, rows_ctas(NT)) int4_rows_kernel(co
           v += s_red[group * wk + k][at_row][n];
           if (SWIGLU) u += s_red[group * wk + k][at_row + 8][n];
         }
-        if (SWIGLU) v = u4::silu_mul(v, u);
+        v *= Act<T>::kUnit;
+        if (SWIGLU) v = u4::silu_mul(v, u * Act<T>::kUnit);
         const int place = first + c0 + n;
         const int64_t at = (int64_t)(p.ids ? s.list[place] : place) * p.n_out + feat;
         if (p.out_f32) static_cast<float*>(p.out)[at] = v;
@@ -838,7 +840,8 @@ __global__ void __launch_bounds__(kMvThreads, 2) int4_down_kernel(const DownPara
       const int tok = i >> 4, f = i & 15;
       float v = s_sum[0][tok][f];
       for (int c = 1; c < p.cluster; ++c) v += *cluster.map_shared_rank(&s_sum[0][tok][f], c);
-      if (strip * 16 + f < p.n_out) static_cast<T*>(p.y)[(int64_t)tok * p.n_out + strip * 16 + f] = Act<T>::from_float(v);
+      if (strip * 16 + f < p.n_out)
+        static_cast<T*>(p.y)[(int64_t)tok * p.n_out + strip * 16 + f] = Act<T>::from_float(v * Act<T>::kUnit);
     }
   }
   cluster.sync();  // no CTA leaves while its sums are read

@@ -569,3 +569,44 @@ def test_decode_batch_with_crowded_experts(T, E, k, H, repeats):
         differ += (mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2)) != first).any()
     assert int(differ) == 0, f"{int(differ)} of 400 calls differ from the first"
     assert mb.device_error() == 0
+
+
+@pytest.mark.parametrize("T,group", [(2, 32), (9, 128), (30, 64)])
+@pytest.mark.parametrize("power", [119, 124, 127])
+def test_grouped_matmul_takes_activations_up_to_the_largest(power, T, group, kernel):
+    """bf16 activations just below the type's largest: sums that fit come out,
+    exactly (all terms are multiples of 2^(power - 14) and their sums below
+    2^(power + 1), so fp32 holds them and no partial sum overflows)."""
+    K, N = 384, 40
+    w, s, wide = weights(2, N, K, group, BF, 3, exact=True)
+    s, wide = s * 2.0 ** -12, wide * 2.0 ** -12
+    x = (torch.randint(-1, 2, (T, K), device=DEV, generator=gen(T)).double() * 2.0 ** power).to(BF)
+    ref, mag = grouped_ref(x, wide, [T - 1, 1])
+    assert float(mag.max()) < 2.0 ** min(power + 1, 128)
+    out = mb.grouped_matmul_int4(x, w, s, torch.tensor([T - 1, 1], device=DEV))
+    assert torch.equal(out, ref.to(BF))
+
+
+@pytest.mark.parametrize("T", [1, 20, 40])
+def test_layer_takes_large_hidden_values(T, kernel):
+    """Rows of h near 2^121 (bf16): the down projection's sums stay finite."""
+    E, k, H, I, group = 16, 3, 256, 384, 128
+    w13, s13, wide13 = weights(E, 2 * I, H, group, BF, 1)
+    w2, s2, wide2 = weights(E, H, I, group, BF, 2)
+    x = (torch.randn((T, H), device=DEV, generator=gen(3)) * 2.0 ** 60).to(BF)
+    wts, ids = routing(T, E, k, 4)
+    ref, bound = layer_ref(x, wide13, wide2, wts, ids, BF)
+    assert 2.0 ** 118 < float(ref.abs().max()) < 2.0 ** 126
+    assert_within(mb.fused_moe_mlp(x, w13, w2, wts, ids, scales=(s13, s2)), ref, bound, BF)
+
+
+@pytest.mark.parametrize("power", [-100, -118, -126])
+def test_grouped_matmul_takes_small_activations(power, kernel):
+    """bf16 activations down to the smallest normal number. Terms are multiples
+    of 2^(power - 2); what a sum may lose is half of bf16's smallest step."""
+    T, K, N = 5, 256, 40
+    w, s, wide = weights(2, N, K, 128, BF, 3, exact=True)
+    x = (torch.randint(-2, 3, (T, K), device=DEV, generator=gen(T)).double() * 2.0 ** power).to(BF)
+    ref, _ = grouped_ref(x, wide, [T - 1, 1])
+    out = mb.grouped_matmul_int4(x, w, s, torch.tensor([T - 1, 1], device=DEV))
+    assert_within(out, ref, torch.zeros_like(ref), BF)
