@@ -806,9 +806,25 @@ int get_encode(EncodeTiledFn* fn) {
   return MOE_OK;
 }
 
-int make_tmap(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, uint64_t rows, uint32_t box_rows) {
+// A 2-D tensor map. The driver's call needs a current context, which a host
+// thread gets with its first runtime call; where this is the first, it is made.
+int encode_tiled(CUtensorMap* m, CUtensorMapDataType dt, const void* ptr, const cuuint64_t (&dims)[2],
+                 const cuuint64_t (&strides)[1], const cuuint32_t (&box)[2], CUtensorMapSwizzle swizzle, CUresult* res) {
   EncodeTiledFn enc;
   MOE_TRY(get_encode(&enc));
+  const cuuint32_t estr[2] = {1, 1};
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    *res = enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (attempt > 0 || (*res != CUDA_ERROR_INVALID_CONTEXT && *res != CUDA_ERROR_NOT_INITIALIZED)) break;
+    int dev = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&dev));
+    MOE_CUDA_TRY(cudaSetDevice(dev));
+  }
+  return MOE_OK;
+}
+
+int make_tmap(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, uint64_t rows, uint32_t box_rows) {
   const int es = dtype_size(dtype);
   CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   if (dtype == MOE_F16) dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -817,10 +833,8 @@ int make_tmap(CUtensorMap* m, const void* ptr, int dtype, uint64_t inner, uint64
   cuuint64_t dims[2] = {inner, rows};
   cuuint64_t strides[1] = {inner * es};
   cuuint32_t box[2] = {(cuuint32_t)(ROW_BYTES / es), box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r;
+  MOE_TRY(encode_tiled(m, dt, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &r));
   if (r != CUDA_SUCCESS)
     return set_error(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu dtype %d", (int)r,
                      (unsigned long long)rows, (unsigned long long)inner, dtype);

@@ -731,15 +731,11 @@ int launch_int4_group(int group, bool swiglu, const Int4Maps& maps, const Int4Pa
 
 // 4-bit words of all experts: boxes of 64 bytes (128 k) by `box_rows` rows.
 int make_tmap_words(CUtensorMap* m, const void* ptr, uint64_t row_bytes, uint64_t rows, uint32_t box_rows) {
-  EncodeTiledFn enc;
-  MOE_TRY(get_encode(&enc));
   cuuint64_t dims[2] = {row_bytes, rows};
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {(cuuint32_t)Q4_RAW_ROW, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r;
+  MOE_TRY(encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B, &r));
   if (r != CUDA_SUCCESS)
     return set_error(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu 4-bit words", (int)r,
                      (unsigned long long)rows, (unsigned long long)row_bytes);

@@ -610,3 +610,56 @@ def test_grouped_matmul_takes_small_activations(power, kernel):
     ref, _ = grouped_ref(x, wide, [T - 1, 1])
     out = mb.grouped_matmul_int4(x, w, s, torch.tensor([T - 1, 1], device=DEV))
     assert_within(out, ref, torch.zeros_like(ref), BF)
+
+
+def in_a_new_thread(call):
+    import threading
+
+    got = []
+
+    def work():
+        try:
+            got.append(call())
+        except Exception as e:  # noqa: BLE001  (handed to the caller)
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    if isinstance(got[0], Exception):
+        raise got[0]
+    return got[0]
+
+
+@pytest.mark.parametrize("entry", ["C", "product", "layer", "bf16"])
+def test_first_cuda_call_of_a_host_thread(entry, kernel):
+    """A thread that has made no CUDA call yet calls the library first."""
+    E, K, N, T = 2, 128, 256, 24
+    w, s, wide = weights(E, N, K, 64, BF, 1, exact=True)
+    w2, s2, _ = weights(E, K, N // 2, 64, BF, 2, exact=True)
+    x = small_ints((T, K), BF, 3)
+    gs = torch.tensor([20, 4], dtype=torch.int32, device=DEV)
+    lib = _lib.load()
+    if entry == "C":
+        out = torch.zeros((T, N), dtype=BF, device=DEV)
+        torch.cuda.synchronize()
+        rc = in_a_new_thread(lambda: (lib.moe_grouped_matmul_int4(
+            x.data_ptr(), _lib.BF16, T, K, w.data_ptr(), s.data_ptr(), 64, E, N, gs.data_ptr(), _lib.I32,
+            out.data_ptr(), None), lib.moe_last_error().decode()))
+        assert rc[0] == 0, rc[1]
+        torch.cuda.synchronize()
+        assert torch.equal(out, grouped_ref(x, wide, [20, 4])[0].to(BF))
+        return
+    if entry == "product":
+        def call():
+            return mb.grouped_matmul_int4(x, w, s, gs)
+    elif entry == "layer":
+        def call():
+            return mb.fused_moe_mlp(x, w, w2, gs, scales=(s, s2))
+    else:
+        a, b = wide.to(BF).transpose(1, 2), torch.zeros((E, K, N // 2), dtype=BF, device=DEV).transpose(1, 2)
+
+        def call():
+            return mb.fused_moe_mlp(x, a, b, gs)
+    torch.cuda.synchronize()
+    assert torch.equal(in_a_new_thread(call), call())
