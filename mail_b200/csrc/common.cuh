@@ -216,6 +216,22 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Lets KFN use up to `smem` bytes of dynamic shared memory, once for each
+// device. The limit belongs to the kernel, for all host threads: set to the size
+// of each launch, one thread would lower it between another's set and launch. So
+// `smem` is the largest size of any launch.
+template <auto KFN>
+int allow_smem(int smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  MOE_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return MOE_OK;
+  MOE_CUDA_TRY(cudaFuncSetAttribute(KFN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return MOE_OK;
+}
+
 // Zeroes `bytes` of device memory on `st` (a kernel launch: moe_rows.cu).
 int zero_fill(void* dst, size_t bytes, cudaStream_t st);
 

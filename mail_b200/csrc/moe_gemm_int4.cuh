@@ -703,7 +703,7 @@ int launch_int4_gemm(const Int4Maps& maps, Int4Params p, int64_t rows_hit, cudaS
   while (p.raw > Sh::kMinRaw && int4_gemm_smem<NARROW>(p.raw, GROUP, p.E) > Q4_MAX_SMEM) p.raw -= Sh::kRawStep;
   const size_t smem = int4_gemm_smem<NARROW>(p.raw, GROUP, p.E);
   auto kfn = int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  MOE_TRY((allow_smem<int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>>((int)Q4_MAX_SMEM)));
   const int64_t items_ub = (ceil_div(p.total_rows, Sh::kRows) + rows_hit) * p.nf;
   const unsigned grid = (unsigned)std::min<int64_t>(num_sms(), items_ub);
   MOE_CUDA_TRY(launch_kernel(kfn, dim3(grid), dim3(Sh::kThreads), smem, st, maps, p));

@@ -907,19 +907,6 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
   return MOE_OK;
 }
 
-// Lets KFN use `smem` bytes of dynamic shared memory, once for each device.
-template <auto KFN>
-int allow_smem(int smem) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  MOE_CUDA_TRY(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-  if (done.load(std::memory_order_relaxed) & bit) return MOE_OK;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(KFN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return MOE_OK;
-}
-
 template <typename T, int GROUP, int NT, bool SWIGLU>
 int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
   constexpr int kSmem = kMvWarps * kRowsDeep * Block4<T, GROUP, rows_tiles(NT)>::kBytes;

@@ -663,3 +663,43 @@ def test_first_cuda_call_of_a_host_thread(entry, kernel):
             return mb.fused_moe_mlp(x, a, b, gs)
     torch.cuda.synchronize()
     assert torch.equal(in_a_new_thread(call), call())
+
+
+def test_tiles_of_different_sizes_from_two_host_threads():
+    """The shared memory of a launch depends on the number of experts; threads
+    whose layers differ do not get in each other's way."""
+    import threading
+
+    lib = _lib.load()
+    before = lib.moe_get_option(_lib.OPT_INT4_GEMM)
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, 1) == 0
+    K, N, T, jobs, streams = 128, 64, 64, [], []
+    for E in (2, 512):
+        w, s, wide = weights(E, N, K, 128, BF, E, exact=True)
+        x = small_ints((T, K), BF, E)
+        gs = torch.tensor([0] * (E - 1) + [T], dtype=torch.int32, device=DEV)
+        out = torch.empty((T, N), dtype=BF, device=DEV)
+        streams.append(torch.cuda.Stream())
+        args = (x.data_ptr(), _lib.BF16, T, K, w.data_ptr(), s.data_ptr(), 128, E, N, gs.data_ptr(), _lib.I32,
+                out.data_ptr(), streams[-1].cuda_stream)
+        jobs.append((args, out, (x.double() @ wide[-1].t()).to(BF), (w, s, x, gs)))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(args):
+        for _ in range(20000):
+            if lib.moe_grouped_matmul_int4(*args) != 0:
+                failed.append(lib.moe_last_error().decode())
+                return
+
+    threads = [threading.Thread(target=work, args=(j[0],)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, before) == 0
+    assert not failed, failed[0]
+    for _, out, ref, _ in jobs:
+        assert torch.equal(out, ref)
+    assert mb.device_error() == 0
