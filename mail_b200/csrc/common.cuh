@@ -219,7 +219,9 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
 // Lets KFN use up to `smem` bytes of dynamic shared memory, once for each
 // device. The limit belongs to the kernel, for all host threads: set to the size
 // of each launch, one thread would lower it between another's set and launch. So
-// `smem` is the largest size of any launch.
+// `smem` is the largest size of any launch (kMaxSmem for a kernel without static
+// shared memory).
+constexpr int kMaxSmem = 227 * 1024;
 template <auto KFN>
 int allow_smem(int smem) {
   static std::atomic<uint64_t> done{0};

@@ -905,7 +905,7 @@ int launch_kind(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
                 const Params& p, int64_t units_ub, cudaStream_t st) {
   const size_t smem = gemm_smem_bytes<PAIR>(p.E, KIND == 2);
   auto kfn = moe_gemm_kernel<KIND, SWIGLU, PAIR>;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  MOE_TRY((allow_smem<moe_gemm_kernel<KIND, SWIGLU, PAIR>>(kMaxSmem)));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.blockDim = dim3(NUM_THREADS);

@@ -43,7 +43,6 @@ constexpr uint32_t Q4_WORD_BYTES = Q4_FEAT * Q4_RAW_ROW;
 constexpr uint32_t q4_raw_bytes(int group) { return Q4_WORD_BYTES + Q4_FEAT * 2 * (128 / group); }  // and scales
 constexpr uint32_t Q4_A_BYTES = Q4_FEAT * ROW_BYTES;
 constexpr int Q4_BOXES = 5;              // boxes of 16, 32, 64, 128 and 256 rows of x
-constexpr size_t Q4_MAX_SMEM = 227 * 1024;
 
 // Rows of x of a tile and pipeline depth. Wide tiles for many rows an expert;
 // narrow ones, with more blocks in flight, where the weights bound the launch.
@@ -700,10 +699,10 @@ template <typename T, int GROUP, bool SWIGLU, bool NARROW>
 int launch_int4_gemm(const Int4Maps& maps, Int4Params p, int64_t rows_hit, cudaStream_t st) {
   using Sh = Int4Shape<NARROW>;
   p.raw = Sh::kMaxRaw;
-  while (p.raw > Sh::kMinRaw && int4_gemm_smem<NARROW>(p.raw, GROUP, p.E) > Q4_MAX_SMEM) p.raw -= Sh::kRawStep;
+  while (p.raw > Sh::kMinRaw && int4_gemm_smem<NARROW>(p.raw, GROUP, p.E) > (size_t)kMaxSmem) p.raw -= Sh::kRawStep;
   const size_t smem = int4_gemm_smem<NARROW>(p.raw, GROUP, p.E);
   auto kfn = int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>;
-  MOE_TRY((allow_smem<int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>>((int)Q4_MAX_SMEM)));
+  MOE_TRY((allow_smem<int4_gemm_kernel<T, GROUP, SWIGLU, NARROW>>(kMaxSmem)));
   const int64_t items_ub = (ceil_div(p.total_rows, Sh::kRows) + rows_hit) * p.nf;
   const unsigned grid = (unsigned)std::min<int64_t>(num_sms(), items_ub);
   MOE_CUDA_TRY(launch_kernel(kfn, dim3(grid), dim3(Sh::kThreads), smem, st, maps, p));

@@ -478,7 +478,7 @@ int launch_swap_kind(const CUtensorMap& tw, const CUtensorMap& tx, const SwapPar
                      cudaStream_t st) {
   const size_t smem = swap_smem_bytes(SWIGLU, p.nmax, p.stages, p.E);
   auto kfn = moe_gemm_swap_kernel<KIND, SWIGLU>;
-  MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  MOE_TRY((allow_smem<moe_gemm_swap_kernel<KIND, SWIGLU>>(kMaxSmem)));
   const int64_t grid = std::min<int64_t>(num_sms(), items_ub);
   if (grid <= 0) return MOE_OK;
   cudaLaunchConfig_t cfg = {};

@@ -205,7 +205,10 @@ int prep_small(const int32_t* topk_ids, int64_t num_tokens, int top_k, int num_e
   MOE_CHECK_ARG(prep_small_fits(S, num_experts), "prep_small: batch too large");
   MOE_CHECK_ARG(hidden % 8 == 0 && zero_a_bytes % 16 == 0 && zero_b_bytes % 16 == 0, "prep_small: bad sizes");
   const int64_t max_tiles = moe_align_capacity(S, num_experts, block_m) / block_m;
-  const size_t smem = ((size_t)2 * S + (size_t)(kPrepWarps + 3) * (num_experts + 1)) * sizeof(int32_t);
+  auto bytes = [](int64_t slots, int experts) {
+    return (int)((2 * slots + (kPrepWarps + 3) * (experts + 1)) * sizeof(int32_t));
+  };
+  const size_t smem = bytes(S, num_experts);
   int64_t grid = ceil_div(S, kPrepWarps);
   const int64_t zero16 = (int64_t)((zero_a_bytes + zero_b_bytes) / 16);
   grid = std::max<int64_t>(grid, ceil_div(zero16, (int64_t)kPrepThreads * 4));
@@ -213,7 +216,7 @@ int prep_small(const int32_t* topk_ids, int64_t num_tokens, int top_k, int num_e
 #define PREP(TT, Q)                                                                                                \
   do {                                                                                                             \
     auto kfn = prep_small_kernel<TT, Q>;                                                                           \
-    if (smem > 48 * 1024) MOE_CUDA_TRY(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+    if (smem > 48 * 1024) MOE_TRY((allow_smem<prep_small_kernel<TT, Q>>(bytes(kPrepMaxSlots, 1024))));              \
     MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)grid), dim3(kPrepThreads), smem, st, topk_ids, S, top_k,          \
                                num_experts, block_m, max_tiles, static_cast<const TT*>(x), hidden, xp, xs,         \
                                sorted_slots, slot_pos, group_sizes, padded_offsets, tile_table,                    \

@@ -444,8 +444,7 @@ extern "C" int moe_tile_schedule(const void* group_sizes, int gs_dtype, int num_
   MOE_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t(1) << 31), "moe_tile_schedule: num_tokens out of range");
   const int64_t grid = moe_tile_grid(num_tokens, num_experts, block_m);
   const size_t smem = 2 * (num_experts + 1) * sizeof(int64_t);
-  if (smem > 48 * 1024)
-    MOE_CUDA_TRY(cudaFuncSetAttribute(tile_schedule_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > 48 * 1024) MOE_TRY(allow_smem<tile_schedule_kernel>(2 * (4096 + 1) * (int)sizeof(int64_t)));
   MOE_CUDA_TRY(launch_kernel(tile_schedule_kernel, dim3(1), dim3(kScanThreads), smem, as_stream(stream),
                              group_sizes, gs_dtype == MOE_I64, num_experts, block_m, grid, tile_expert,
                              tile_row_start, tile_row_count, tile_table));
@@ -495,9 +494,9 @@ int launch_align_small(const int32_t* topk_ids, int64_t S, int E, int block_m, i
                        int32_t* slot_pos, int32_t* group_sizes, int32_t* padded_offsets, int32_t* tile_table,
                        cudaStream_t st) {
   const int64_t max_tiles = moe_align_capacity(S, E, block_m) / block_m;
-  const size_t smem = ((size_t)(kScanThreads / 32) + 3) * (E + 1) * sizeof(int32_t);
-  if (smem > 48 * 1024)
-    MOE_CUDA_TRY(cudaFuncSetAttribute(align_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  auto bytes = [](int experts) { return (int)((kScanThreads / 32 + 3) * (experts + 1) * sizeof(int32_t)); };
+  const size_t smem = bytes(E);
+  if (smem > 48 * 1024) MOE_TRY(allow_smem<align_small_kernel>(bytes(1024)));
   MOE_CUDA_TRY(launch_kernel(align_small_kernel, dim3(1), dim3(kScanThreads), smem, st, topk_ids, S, E, block_m,
                              max_tiles, sorted_slots, slot_pos, group_sizes, padded_offsets, tile_table));
   MOE_LAUNCH_CHECK("align_small_kernel");
