@@ -100,11 +100,11 @@ def weights_from_checkpoint(gate_proj, up_proj, down_proj, device=None, dtype=No
     layout the kernels' TMA reads) on `device` (default: the tensors' own),
     cast to `dtype` if given — no concatenated or stacked intermediate.
 
-    quantize=True or "int8" (CUDA device) converts to w8a8 weights with
-    per-output-channel scales (quantize_weights_int8), "int4" to 4-bit weights
-    with scales for groups of group_size (quantize_weights_int4); both return
-    (w13_q, w2_q, scales); otherwise (w13, w2)."""
-    if quantize not in (False, True, "int8", "int4"):
+    quantize=True (or anything true) or "int8" (CUDA device) converts to w8a8
+    weights with per-output-channel scales (quantize_weights_int8), "int4" to
+    4-bit weights with scales for groups of group_size (quantize_weights_int4);
+    both return (w13_q, w2_q, scales); otherwise (w13, w2)."""
+    if isinstance(quantize, str) and quantize not in ("", "int8", "int4"):
         raise ValueError(f"weights_from_checkpoint: quantize must be a bool, 'int8' or 'int4', not {quantize!r}")
     E = len(gate_proj)
     if len(up_proj) != E or len(down_proj) != E or E == 0:

@@ -135,3 +135,23 @@ def test_checkpoint_quantize_argument():
         mb.weights_from_checkpoint(z, z, z, quantize="int3")
     with pytest.raises(ValueError, match="CUDA"):
         mb.weights_from_checkpoint(z, z, z, quantize="int4", group_size=64)
+
+
+@pytest.mark.parametrize("quantize", [None, 0, "", [], 2, (1,), "int8"])
+def test_checkpoint_quantize_is_taken_by_its_truth(quantize):
+    """Any value that is no string is taken by its truth, as before there were
+    names for the types; what asks for int8 gets as far as needing the device."""
+    z = torch.zeros((1, 64, 64), dtype=BF)
+    if quantize:
+        with pytest.raises(ValueError, match="CUDA"):
+            mb.weights_from_checkpoint(z, z, z, quantize=quantize)
+    else:
+        w13, w2 = mb.weights_from_checkpoint(z, z, z, quantize=quantize)
+        assert w13.shape == (1, 64, 128) and w2.shape == (1, 64, 64) and w13.dtype == BF
+
+
+def test_checkpoint_names_that_mean_nothing_are_refused():
+    z = torch.zeros((1, 64, 64), dtype=BF)
+    for name in ("int2", "fp8", "INT4"):
+        with pytest.raises(ValueError, match="quantize"):
+            mb.weights_from_checkpoint(z, z, z, quantize=name)
