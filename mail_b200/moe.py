@@ -380,17 +380,18 @@ def fused_moe_mlp(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, group_si
     """
     del BLOCK_M, BLOCK_N, BLOCK_N2, BLOCK_K
     compiling = torch.compiler.is_compiling()
-    s13, s2 = scales if scales is not None else (None, None)
     if topk_ids is None:
         if w13.dtype == torch.uint8:
             if scales is None:
                 raise ValueError("fused_moe_mlp: 4-bit weights need scales=(w13_scale, w2_scale)")
+            s13, s2 = scales
             if compiling:
                 return torch.ops.mail_b200.fused_moe_mlp_int4(x, w13, w2, group_sizes_or_topk_weights, s13, s2)
             return int4.fused_mlp(x, w13, w2, group_sizes_or_topk_weights, s13, s2)
         if compiling:
             return torch.ops.mail_b200.fused_moe_mlp(x, w13, w2, group_sizes_or_topk_weights)
         return _prerouted_impl(x, w13, w2, group_sizes_or_topk_weights)
+    s13, s2 = scales if scales is not None else (None, None)
     if compiling:
         return torch.ops.mail_b200.fused_experts(x, w13, w2, group_sizes_or_topk_weights, topk_ids, s13, s2)
     return _topk_impl(x, w13, w2, group_sizes_or_topk_weights, topk_ids, s13, s2)

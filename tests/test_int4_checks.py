@@ -155,3 +155,10 @@ def test_checkpoint_names_that_mean_nothing_are_refused():
     for name in ("int2", "fp8", "INT4"):
         with pytest.raises(ValueError, match="quantize"):
             mb.weights_from_checkpoint(z, z, z, quantize=name)
+
+
+@pytest.mark.parametrize("scales", [(), (None,), (None, None, None), torch.zeros(3)])
+def test_pre_routed_call_with_dense_weights_does_not_read_scales(scales):
+    x, w13, w2 = (torch.zeros(s, dtype=BF) for s in ((4, 64), (2, 64, 128), (2, 64, 64)))
+    with pytest.raises(ValueError, match="CUDA tensors only"):  # past the argument
+        mb.fused_moe_mlp(x, w13, w2, torch.tensor([2, 2]), scales=scales)
