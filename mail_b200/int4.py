@@ -141,9 +141,12 @@ def _check_weight(name: str, dtype: torch.dtype, w: torch.Tensor, scale: torch.T
     return group_size
 
 
-def _counts(name: str, group_sizes: torch.Tensor, E: int) -> torch.Tensor:
+def _check_counts(name: str, group_sizes: torch.Tensor, E: int) -> None:
     if group_sizes.numel() != E:
         raise ValueError(f"{name}: group_sizes must have E entries")
+
+
+def _counts(group_sizes: torch.Tensor) -> torch.Tensor:
     if group_sizes.dtype not in (torch.int32, torch.int64):
         group_sizes = group_sizes.to(torch.int64)
     return group_sizes.contiguous()
@@ -166,15 +169,22 @@ def grouped_matmul_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     return _grouped_impl(x, w, scale, group_sizes)
 
 
-def _grouped_impl(x, w, scale, group_sizes):
+def _check_grouped(x, w, scale, group_sizes) -> int:
+    """Group size of a grouped product's weights, its arguments checked."""
     name = "grouped_matmul_int4"
-    dev = _one_device(name, x, w, scale, group_sizes)
     if x.dim() != 2:
         raise ValueError(f"{name}: expected x [T, K]")
+    group_size = _check_weight(name, x.dtype, w, scale, x.shape[1])
+    _check_counts(name, group_sizes, w.shape[0])
+    return group_size
+
+
+def _grouped_impl(x, w, scale, group_sizes):
+    dev = _one_device("grouped_matmul_int4", x, w, scale, group_sizes)
+    group_size = _check_grouped(x, w, scale, group_sizes)
     T, K = x.shape
-    group_size = _check_weight(name, x.dtype, w, scale, K)
     E, _, N = w.shape
-    gs = _counts(name, group_sizes, E)
+    gs = _counts(group_sizes)
     x, wk, scale = x.contiguous(), _kmajor(w), scale.contiguous()
     out = torch.empty((T, N), dtype=x.dtype, device=dev)
     _launch(dev, "moe_grouped_matmul_int4", x.data_ptr(), _CODES[x.dtype], T, K, wk.data_ptr(), scale.data_ptr(),
@@ -182,19 +192,25 @@ def _grouped_impl(x, w, scale, group_sizes):
     return out
 
 
-def _layer_weights(x, w13, w2, w13_scale, w2_scale):
-    """(E, H, I, group size, K-major w13, scales, K-major w2, scales), checked."""
+def check_layer(x, w13, w2, w13_scale, w2_scale) -> int:
+    """Group size of a layer's 4-bit weights, types and scales checked (the
+    shapes of x, w13 and w2 by _check_shapes)."""
     name = "fused_moe_mlp"
     if w13_scale is None or w2_scale is None:
         raise ValueError(f"{name}: 4-bit weights need scales=(w13_scale, w2_scale)")
     if w2.dtype != torch.uint8:
         raise TypeError(f"{name}: w13 and w2 must both be 4-bit (uint8)")
-    H = x.shape[1]
-    E, _, two_i = w13.shape
-    group = _check_weight(name, x.dtype, w13, w13_scale, H)
-    if _check_weight(name, x.dtype, w2, w2_scale, two_i // 2) != group:
+    group = _check_weight(name, x.dtype, w13, w13_scale, x.shape[1])
+    if _check_weight(name, x.dtype, w2, w2_scale, w13.shape[2] // 2) != group:
         raise ValueError(f"{name}: w13 and w2 must share a group size")
-    return E, H, two_i // 2, group, _kmajor(w13), w13_scale.contiguous(), _kmajor(w2), w2_scale.contiguous()
+    return group
+
+
+def _layer_weights(x, w13, w2, w13_scale, w2_scale):
+    """(E, H, I, group size, K-major w13, scales, K-major w2, scales), checked."""
+    group = check_layer(x, w13, w2, w13_scale, w2_scale)
+    E, _, two_i = w13.shape
+    return E, x.shape[1], two_i // 2, group, _kmajor(w13), w13_scale.contiguous(), _kmajor(w2), w2_scale.contiguous()
 
 
 def fused_experts(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
@@ -223,7 +239,8 @@ def fused_mlp(x, w13, w2, group_sizes, w13_scale, w2_scale):
     E, H, inter, group, a, sa, b, sb = _layer_weights(x, w13, w2, w13_scale, w2_scale)
     dev = _one_device("fused_moe_mlp", x, w13, w2, group_sizes, w13_scale, w2_scale)
     x = x.contiguous()
-    gs = _counts("fused_moe_mlp", group_sizes, E)
+    _check_counts("fused_moe_mlp", group_sizes, E)
+    gs = _counts(group_sizes)
     T = x.shape[0]
     out = torch.empty((T, H), dtype=x.dtype, device=dev)
     size = _lib.query("moe_fused_mlp_int4_workspace_size", T, inter, E)
@@ -243,8 +260,8 @@ def _op_prerouted(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, group_si
 @_op_prerouted.register_fake
 def _(x, w13, w2, group_sizes, w13_scale, w2_scale):
     T, H, E, _ = _check_shapes(x, w13, w2)
-    if group_sizes.numel() != E:
-        raise ValueError("fused_moe_mlp: group_sizes must have E entries")
+    check_layer(x, w13, w2, w13_scale, w2_scale)
+    _check_counts("fused_moe_mlp", group_sizes, E)
     return x.new_empty((T, H))
 
 
@@ -255,5 +272,5 @@ def _op_grouped(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, group_siz
 
 @_op_grouped.register_fake
 def _(x, w, scale, group_sizes):
-    _check_weight("grouped_matmul_int4", x.dtype, w, scale, x.shape[1])
+    _check_grouped(x, w, scale, group_sizes)
     return x.new_empty((x.shape[0], w.shape[2]))

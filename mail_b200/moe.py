@@ -344,6 +344,8 @@ def _(x, w13, w2, topk_weights, topk_ids, w13_scale, w2_scale):
     T, H, _, _ = _check_shapes(x, w13, w2)
     if topk_weights.shape != topk_ids.shape or topk_ids.dim() != 2 or topk_ids.shape[0] != T:
         raise ValueError("fused_moe_mlp: topk_weights/topk_ids must both be [T, k]")
+    if w13.dtype == torch.uint8:
+        int4.check_layer(x, w13, w2, w13_scale, w2_scale)
     return x.new_empty((T, H))
 
 
@@ -441,6 +443,8 @@ def _op_from_logits(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, router
 @_op_from_logits.register_fake
 def _(x, w13, w2, router_logits, top_k, scoring, renormalize, w13_scale, w2_scale):
     T, H, _, _ = _check_logits(x, w13, w2, router_logits, top_k, scoring)
+    if w13.dtype == torch.uint8:
+        int4.check_layer(x, w13, w2, w13_scale, w2_scale)
     return (x.new_empty((T, H)), x.new_empty((T, top_k), dtype=torch.float32),
             x.new_empty((T, top_k), dtype=torch.int32))
 

@@ -162,3 +162,58 @@ def test_pre_routed_call_with_dense_weights_does_not_read_scales(scales):
     x, w13, w2 = (torch.zeros(s, dtype=BF) for s in ((4, 64), (2, 64, 128), (2, 64, 64)))
     with pytest.raises(ValueError, match="CUDA tensors only"):  # past the argument
         mb.fused_moe_mlp(x, w13, w2, torch.tensor([2, 2]), scales=scales)
+
+
+def _fake(*shapes):
+    return [torch.empty(s, dtype=d) for s, d in shapes]
+
+
+@pytest.mark.parametrize("change,err,needle", [
+    (dict(x=((256,), BF)), ValueError, "x \\[T, K\\]"),
+    (dict(x=((2, 6, 256), BF)), ValueError, "x \\[T, K\\]"),
+    (dict(gs=((3,), torch.int64)), ValueError, "E entries"),
+    (dict(gs=((0,), torch.int64)), ValueError, "E entries"),
+    (dict(w=((4, 64, 256), torch.uint8)), ValueError, "K = 256"),
+    (dict(s=((4, 256, 2), HF)), TypeError, "share"),
+])
+def test_registered_product_refuses_when_traced(change, err, needle):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    args = dict(x=((6, 256), BF), w=((4, 128, 256), torch.uint8), s=((4, 256, 2), BF), gs=((4,), torch.int64))
+    with FakeTensorMode():
+        assert tuple(torch.ops.mail_b200.grouped_matmul_int4(*_fake(*args.values())).shape) == (6, 256)
+        with pytest.raises(err, match=needle):
+            torch.ops.mail_b200.grouped_matmul_int4(*_fake(*{**args, **change}.values()))
+
+
+@pytest.mark.parametrize("change,err,needle", [
+    (dict(x=((6, 256), torch.float32)), TypeError, "bf16 or fp16"),
+    (dict(w2=((4, 64, 256), BF)), TypeError, "both be 4-bit"),
+    (dict(s13=((4, 256, 3), BF)), ValueError, "do not fit"),
+    (dict(s13=((4, 256, 2), HF)), TypeError, "share"),
+    (dict(s2=((4, 128, 1), BF)), ValueError, "do not fit"),
+    (dict(s2=((4, 256, 2), BF)), ValueError, "share a group size"),
+    (dict(s2=None), ValueError, "need scales"),
+])
+@pytest.mark.parametrize("form", ["top-k", "logits", "pre-routed"])
+def test_registered_layers_refuse_when_traced(form, change, err, needle):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    args = dict(x=((6, 256), BF), w13=((4, 128, 256), torch.uint8), w2=((4, 64, 256), torch.uint8),
+                s13=((4, 256, 2), BF), s2=((4, 256, 1), BF))
+    ops = torch.ops.mail_b200
+
+    def call(a):
+        x, w13, w2, s13, s2 = (None if v is None else torch.empty(v[0], dtype=v[1]) for v in a.values())
+        if form == "top-k":
+            return ops.fused_experts(x, w13, w2, torch.empty((6, 2)), torch.empty((6, 2), dtype=torch.int32), s13, s2)
+        if form == "logits":
+            return ops.fused_experts_from_logits(x, w13, w2, torch.empty((6, 4)), 2, "softmax", True, s13, s2)[0]
+        return ops.fused_moe_mlp_int4(x, w13, w2, torch.empty(4, dtype=torch.int64), s13, s2)
+
+    if form == "pre-routed" and change.get("s2", 0) is None:
+        return  # that operator's scales are not optional
+    with FakeTensorMode():
+        assert tuple(call(args).shape) == (6, 256)
+        with pytest.raises(err, match=needle):
+            call({**args, **change})
