@@ -405,8 +405,9 @@ MOE_API int moe_fused_expert_rows(const void* x, int x_dtype, int64_t rows, int6
  * in a fixed order, so results do not differ from run to run.
  *
  * Few rows an expert (MOE_OPT_INT4_GEMM) run without rounding a weight; the
- * tensor-core tiles round each (q - 8) s once to x's type. A row of x that holds
- * an infinity gives infinities or NaN in its own row of out only.
+ * tensor-core tiles round each (q - 8) s once to x's type, so in fp16 a weight
+ * beyond 65504 (scales above 8188) is infinite there. A row of x that holds an
+ * infinity gives infinities or NaN in its own row of out only.
  * -------------------------------------------------------------------------- */
 MOE_API int moe_quant_int4_groups(const void* src, int src_dtype, int64_t rows, int64_t cols, int group_size,
                                   uint8_t* dst, void* dst_scale, int scale_dtype, void* stream);

@@ -12,6 +12,10 @@ contiguous [E, 2I, H / 2] bytes with scales [E, 2I, H / group_size], and w2 is
 [E, I / 2, H] with scales [E, H, I / group_size]. `fused_moe_mlp` and
 `fused_moe_mlp_from_logits` take such weights with scales=(w13_scale, w2_scale).
 
+Up to eight rows an expert on average are multiplied without rounding a weight;
+with more, each weight is rounded once to the activations' type (in fp16 one
+beyond 65504, from a scale above 8188, is infinite there).
+
 Every op runs the kernels of libmoe_b200.so on the current stream of its
 tensors' device; there is no CPU or PyTorch fallback.
 """

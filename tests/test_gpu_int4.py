@@ -703,3 +703,107 @@ def test_tiles_of_different_sizes_from_two_host_threads():
     for _, out, ref, _ in jobs:
         assert torch.equal(out, ref)
     assert mb.device_error() == 0
+
+
+def full_scales(shape, bits, dtype, seed):
+    """Scales with all `bits` significant bits in one binade: multiples of
+    2^(1 - bits) in [1, 2)."""
+    m = torch.randint(2 ** (bits - 1), 2 ** bits, shape, device=DEV, generator=gen(seed))
+    return (m.double() * 2.0 ** (1 - bits)).to(dtype)
+
+
+@pytest.fixture
+def row_kernels():
+    lib = _lib.load()
+    before = lib.moe_get_option(_lib.OPT_INT4_GEMM)
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, 0) == 0
+    yield
+    assert mb.device_error() == 0
+    assert lib.moe_set_option(_lib.OPT_INT4_GEMM, before) == 0
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF, 8), (HF, 11)])
+@pytest.mark.parametrize("K,N,group,sizes", [(32, 70, 32, [3]), (384, 40, 128, [1, 0, 2]), (384, 33, 64, [9, 17]),
+                                             (512, 50, 32, [40, 1])])
+def test_row_kernels_round_no_weight(dtype, bits, K, N, group, sizes, row_kernels):
+    """Scales with a full significand: (q - 8) s needs more bits than the
+    activations' type has. All terms are multiples of 2^(1 - bits), and the sums
+    of their magnitudes below 2^24 of these, so fp32 holds every sum: the output
+    has to be the exact result, rounded once."""
+    E, T = len(sizes), sum(sizes)
+    w, _, wide = weights(E, N, K, group, dtype, K + N, exact=False)
+    q = torch.stack((w.transpose(1, 2) & 15, w.transpose(1, 2) >> 4), dim=-1).view(E, N, K)
+    s = full_scales((E, N, K // group), bits, dtype, N)
+    wide = (q.double() - 8) * s.double().repeat_interleave(group, dim=2)
+    assert bool((wide.to(dtype).double() != wide).any())
+    x = small_ints((T, K), dtype, T)
+    ref, mag = grouped_ref(x, wide, sizes)
+    assert float(mag.max()) * 2 ** (bits - 1) < 2 ** 24
+    out = mb.grouped_matmul_int4(x, w, s, torch.tensor(sizes, dtype=torch.int32, device=DEV))
+    assert torch.equal(out, ref.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,E,k", [(1, 4, 1), (3, 4, 4), (20, 8, 4), (32, 32, 8), (40, 6, 3)])
+def test_decode_layer_rounds_no_weight(dtype, T, E, k, row_kernels):
+    """A layer whose h is exact (gates are 128, where silu(g) = g; h = 128 u with
+    |u| <= 32 whole) and whose down weights need more bits than the type has. The
+    terms are multiples of 2^-3, all sums below 2^21."""
+    H, I, group = 64, 64, 32
+    g = gen(T)
+    q13 = torch.randint(0, 16, (E, 2 * I, H), device=DEV, generator=g)
+    q13[:, :I] = 8
+    q13[:, :I, 0] = 12   # gate = 4 * 2 * x[0]
+    q13[:, I:, 0] = 8
+    s13 = torch.ones((E, 2 * I, H // group), device=DEV)
+    s13[:, :I] = 2
+    w13 = (q13[..., 0::2] | (q13[..., 1::2] << 4)).to(torch.uint8).transpose(1, 2)
+    w2, _, _ = weights(E, H, I, group, dtype, 2)
+    q2 = torch.stack((w2.transpose(1, 2) & 15, w2.transpose(1, 2) >> 4), dim=-1).view(E, H, I)
+    s2 = full_scales((E, H, I // group), 8, dtype, 3)
+    wide2 = (q2.double() - 8) * s2.double().repeat_interleave(group, dim=2)
+    x = torch.zeros((T, H), device=DEV)
+    x[:, 1:5] = torch.randint(-1, 2, (T, 4), device=DEV, generator=g).float()
+    x[:, 0] = 16
+    _, ids = routing(T, E, k, 4)
+    wts = torch.tensor([0.5, 0.25, 0.125], device=DEV)[torch.randint(0, 3, (T, k), device=DEV, generator=g)]
+    ref = torch.zeros((T, H), dtype=torch.float64, device=DEV)
+    mag = torch.zeros_like(ref)
+    for j in range(k):
+        u = torch.einsum("th,tnh->tn", x.double(), q13[ids[:, j].long(), I:].double() - 8)
+        assert float(u.abs().max()) <= 32
+        o = torch.einsum("ti,tni->tn", 128 * u, wide2[ids[:, j].long()])
+        m = torch.einsum("ti,tni->tn", 128 * u.abs(), wide2[ids[:, j].long()].abs())
+        ref += wts[:, j:j + 1].double() * o
+        mag += wts[:, j:j + 1].double() * m
+    assert float(mag.max()) * 2 ** 3 < 2 ** 24
+    y = mb.fused_moe_mlp(x.to(dtype), w13, w2, wts, ids, scales=(s13.to(dtype), s2))
+    assert torch.equal(y, ref.to(dtype))
+
+
+def test_grouped_matmul_spreads_an_infinity_over_its_row_only(kernel):
+    """q = 8 makes 0 * inf = NaN of it, every other weight an infinity; rows of
+    the same tile keep their values."""
+    w, s, wide = weights(2, 64, 256, 128, BF, 5, exact=True)
+    x = small_ints((20, 256), BF, 3)
+    ref, _ = grouped_ref(x, wide, [9, 11])
+    for r, c, v in ((2, 0, float("inf")), (15, 200, float("inf")), (19, 255, -float("inf"))):
+        x[r, c] = v
+    out = mb.grouped_matmul_int4(x, w, s, torch.tensor([9, 11], device=DEV))
+    rows = [r for r in range(20) if r not in (2, 15, 19)]
+    assert torch.equal(out[rows], ref.to(BF)[rows])
+    assert not bool(torch.isfinite(out[[2, 15, 19]]).any())
+
+
+def test_grouped_matmul_takes_fp16_scales_up_to_8188(kernel):
+    """-8 * 8188 is fp16's largest number: up to there the tiles hold every
+    weight, and exactly where the step is a power of two."""
+    K, N, T = 64, 40, 12
+    q = torch.tensor([0, 4, 6, 7, 8, 9, 10, 12], device=DEV)[torch.randint(0, 8, (N, K), device=DEV, generator=gen(5))]
+    s = torch.full((1, N, K // 32), 8188.0, dtype=HF, device=DEV)
+    w = (q[:, 0::2] | (q[:, 1::2] << 4)).to(torch.uint8).view(1, N, K // 2).transpose(1, 2)
+    wide = (q.double() - 8) * 8188
+    assert torch.equal(wide.to(HF).double(), wide) and float(wide.min()) == -65504
+    x = (small_ints((T, K), HF, 3).double() * 2.0 ** -8).to(HF)
+    ref = x.double() @ wide.t()
+    assert torch.equal(mb.grouped_matmul_int4(x, w, s, torch.tensor([T], device=DEV)), ref.to(HF))
