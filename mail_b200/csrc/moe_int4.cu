@@ -529,8 +529,8 @@ __device__ __forceinline__ void group_barrier(int id, int threads) {
 // Blocks of 128 k whose words a warp has in flight.
 constexpr int kRowsDeep = 4;
 // Weight tiles of a warp and CTAs of an SM.
-__host__ __device__ constexpr int rows_tiles(int nt) { return 2; }
-__host__ __device__ constexpr int rows_ctas(int nt) { return 2; }
+constexpr int kRowsTiles = 2;
+constexpr int kRowsCtas = 2;
 
 // A place in a warp's run of work: the unit (an expert's strip), the chunk of
 // the expert's rows, the block of K.
@@ -540,11 +540,11 @@ struct RowsWork {
 };
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
-__global__ void __launch_bounds__(kMvThreads, rows_ctas(NT)) int4_rows_kernel(const MvParams p) {
+__global__ void __launch_bounds__(kMvThreads, kRowsCtas) int4_rows_kernel(const MvParams p) {
   pdl_begin();
   constexpr int kWords = GROUP / 32;      // 32-bit words a lane loads of a row and group
   constexpr int kTokens = 8 * NT;
-  constexpr int MT = rows_tiles(NT);
+  constexpr int MT = kRowsTiles;
   constexpr int kFeat = (SWIGLU ? 8 : 16) * MT;  // output features of a strip
   using B = Block4<T, GROUP, MT>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -909,9 +909,9 @@ int launch_dequant(const void* src, const void* scale, int64_t n8, int group, vo
 
 template <typename T, int GROUP, int NT, bool SWIGLU>
 int launch_rows_nt(MvParams p, int64_t rows, cudaStream_t st) {
-  constexpr int kSmem = kMvWarps * kRowsDeep * Block4<T, GROUP, rows_tiles(NT)>::kBytes;
-  const int64_t units = ceil_div(p.n_out, (SWIGLU ? 8 : 16) * rows_tiles(NT)) * std::min<int64_t>(p.E, rows);
-  const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), rows_ctas(NT) * num_sms());
+  constexpr int kSmem = kMvWarps * kRowsDeep * Block4<T, GROUP, kRowsTiles>::kBytes;
+  const int64_t units = ceil_div(p.n_out, (SWIGLU ? 8 : 16) * kRowsTiles) * std::min<int64_t>(p.E, rows);
+  const int64_t ctas = std::min<int64_t>(units * ceil_div(p.K, 1024), kRowsCtas * num_sms());
   auto kfn = int4_rows_kernel<T, GROUP, NT, SWIGLU>;
   MOE_TRY((allow_smem<int4_rows_kernel<T, GROUP, NT, SWIGLU>>(kSmem)));
   MOE_CUDA_TRY(launch_kernel(kfn, dim3((unsigned)ctas), dim3(kMvThreads), kSmem, st, p));
