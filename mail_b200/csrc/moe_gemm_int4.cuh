@@ -57,6 +57,10 @@ constexpr int Q4_BOXES = 5;              // boxes of 16, 32, 64, 128 and 256 row
 // kMaxRaw of them, so that the same holds there: three sets know the blocks of
 // words up to five before the next one multiplied; four sets come to every
 // second block, and an even number of slots makes a slot's last use their own.
+// The host takes as many as shared memory holds: wide tiles four for groups of
+// 128 over up to 91 experts, else two (8192 rows over eight experts of 4096 x
+// 14336 with two: 799 us against 743; groups of 64 and 32 take 825 and 972);
+// narrow ones nine, or eight for groups of 32 over more than 91 experts.
 // Narrow tiles have two stages for each set: it decodes one while the other
 // multiplies. Wide ones multiply longer than they decode, and four sets with a
 // stage each keep up.
@@ -71,10 +75,10 @@ struct Int4Shape {
   static constexpr int kThreads = 32 * (8 + 4 * kSets);
 };
 // Narrow tiles up to this many rows an expert on average. Narrow in us against
-// wide in us, 64 experts of 2048 x 1536: 32: 59 / 66, 48: 61 / 68, 64: 81 / 70;
-// 16 experts of 4096 x 4096: 32: 71 / 79, 48: 73 / 83, 64: 103 / 85. Narrow as
-// well where all of them run at once (777 rows, 5 experts of 1056 x 1001: 18.7 /
-// 20.6; not so, 600 rows, 2 experts of 7168 x 2048: 62 / 47).
+// wide in us, 64 experts of 2048 x 1536: 32: 58 / 63, 48: 60 / 65, 64: 79 / 67;
+// 16 experts of 4096 x 4096: 32: 70 / 79, 48: 72 / 82, 64: 102 / 84. Narrow as
+// well where all of them run at once (777 rows, 5 experts of 1056 x 1001: 12.6 /
+// 17.6; not so, 600 rows, 2 experts of 7168 x 2048: 60 / 40).
 constexpr int64_t kInt4NarrowRows = 48;
 
 struct Int4Maps {

@@ -969,7 +969,10 @@ int launch_down_any(const DownParams& p, int dtype, int group, cudaStream_t st) 
 // Tensor-core tiles or the row kernels (MOE_OPT_INT4_GEMM). Rows in us against
 // tiles in us, by rows an expert, 128 experts of 2048 x 1536: 2: 60 / 87,
 // 4: 90 / 98, 8: 95 / 99, 12: 125 / 99; 8 experts of 4096 x 14336: 2: 72 / 105,
-// 8: 112 / 112, 12: 136 / 111.
+// 8: 112 / 112, 12: 136 / 111. The counts are on the device, so the rule goes by
+// the mean: with 8 on average and one expert of 100 or 500 rows the row kernels
+// take 202 and 701 us, the tiles 97 and 99 (a caller that knows its routing to be
+// that uneven sets the option).
 constexpr int64_t kRowsPerExpert = 8;
 bool use_gemm(int64_t rows, int64_t n_out, int64_t w_rows, int E) {
   const int opt = moe_get_option(MOE_OPT_INT4_GEMM);
