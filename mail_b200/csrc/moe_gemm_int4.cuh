@@ -60,7 +60,8 @@ constexpr int Q4_BOXES = 5;              // boxes of 16, 32, 64, 128 and 256 row
 // The host takes as many as shared memory holds: wide tiles four for groups of
 // 128 over up to 91 experts, else two (8192 rows over eight experts of 4096 x
 // 14336 with two: 799 us against 743; groups of 64 and 32 take 825 and 972);
-// narrow ones nine, or eight for groups of 32 over more than 91 experts.
+// narrow ones nine, or eight for groups of 32, 64 and 128 over more than 91, 667
+// and 955 experts.
 // Narrow tiles have two stages for each set: it decodes one while the other
 // multiplies. Wide ones multiply longer than they decode, and four sets with a
 // stage each keep up.

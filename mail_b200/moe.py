@@ -372,8 +372,8 @@ def fused_moe_mlp(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, group_si
     Both forms take 4-bit weights with group scales (quantize_weights_int4):
     uint8 w13 [E, H / 2, 2I] and w2 [E, I / 2, H] with scales=(w13_scale
     [E, 2I, H / group_size], w2_scale [E, H, I / group_size]) in x's type
-    (bf16 or fp16). Their combine adds a token's rows in slot order, so
-    results do not differ from run to run.
+    (bf16 or fp16). Their sums are added in a fixed order, so results do
+    not differ from run to run.
 
     Under torch.compile the call is one operator (torch.ops.mail_b200.
     fused_moe_mlp / fused_moe_mlp_int4 / fused_experts); eager calls go straight to the library.
